@@ -43,8 +43,8 @@ def parse_args(argv=None):
                     help="bf16 weights with an exact fp32 master stored split (low halves + bf16 moments as optimizer state)")
     ap.add_argument("--layers", type=int, default=None, help="debug only: cut the model (the result is not a valid bench)")
     ap.add_argument("--kernels", default=None, help="kernel lane override (e.g. baseline)")
-    ap.add_argument("--linear-precision", default="bf16", choices=["bf16", "fp8"],
-                    help="fp8: e4m3 forward projections (an extra data point; the headline metric is the bf16 run)")
+    ap.add_argument("--linear-precision", default="bf16", choices=["bf16", "fp8", "mxfp4"],
+                    help="fp8 / mxfp4: e4m3 or 4-bit forward projections (an extra data point; the headline metric is the bf16 run)")
     ap.add_argument("--no-profile", action="store_true", help="plan from roofline seeds instead of measured task costs")
     ap.add_argument("--parallel", default=None, help="fsdp | zero3 | zero1 (default: fsdp when --gpus > 1)")
     ap.add_argument("--plan-only", action="store_true",
@@ -183,7 +183,7 @@ def bench_ours(a) -> dict:
     out = {
         "metric": "train_tokens_per_s", "value": value, "unit": "tokens/s", "n_gpus": world, "steps": a.steps,
         "warmup": a.warmup, "ms_per_step": dev_s / a.steps * 1e3, "higher_is_better": True, "scaling": "weak",
-        "vs_baseline": value / BASELINE_TOK_S, "dtype": "bf16" if a.linear_precision == "bf16" else "bf16 (fp8 forward projections)",
+        "vs_baseline": value / BASELINE_TOK_S, "dtype": "bf16" if a.linear_precision == "bf16" else f"bf16 ({a.linear_precision} forward projections)",
         "data": "synthetic", "impl": "ours",
         "config": {"model": a.preset + (f"-cut{a.layers}L" if a.layers else ""), "global_batch": tokens_step * world // a.seq_len,
                    "seq_len": a.seq_len, "tokens_per_step": tokens_step * world,

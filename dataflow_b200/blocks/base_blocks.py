@@ -214,6 +214,7 @@ class OptimizerStep(_Base):
         eps, wd = hy.get("eps", 1e-8), hy.get("weight_decay", 0.0)
         rule = hy.get("optimizer", "adamw")
         only = tuple(hy.get("train_only") or ())
+        eight: dict[tuple, list] = {}               # fields with 8-bit moments, by master form: one launch for each form
         for f in wl.fields:
             if f.name not in g:
                 continue            # frozen field: no gradient storage, no update
@@ -221,7 +222,10 @@ class OptimizerStep(_Base):
                 continue            # the run updates a named subset of fields only (e.g. an indexer warm-up)
             wf, gf = w[f.name], g[f.name]
             f_wd = wd if (f.kind in ("matrix", "embedding") or hy.get("wd_all")) else 0.0
-            if rule == "adamw" and f"{f.name}.mlo" in o:
+            if rule == "adamw" and f"{f.name}.s0_scale" in o:
+                extra = next((k for k in ("master", "mlo") if f"{f.name}.{k}" in o), None)
+                eight.setdefault((extra, wf.dtype, gf.dtype), []).append((f.name, wf, gf, f_wd))
+            elif rule == "adamw" and f"{f.name}.mlo" in o:
                 self.K.adamw_split_step(wf.reshape(-1), o[f"{f.name}.mlo"].reshape(-1), gf.reshape(-1),
                                         o[f"{f.name}.s0"].reshape(-1), o[f"{f.name}.s1"].reshape(-1), lr, b1, b2, eps, f_wd, step)
             elif rule == "adamw":
@@ -238,6 +242,12 @@ class OptimizerStep(_Base):
                 continue
             else:
                 raise KeyError(f"unknown optimizer rule {rule!r}")
+        for (extra, _, _), fs in eight.items():
+            slot = lambda part: [o[f"{name}.{part}"].reshape(-1) for name, _, _, _ in fs]
+            self.K.lowbit.adamw_multi_step([w_.reshape(-1) for _, w_, _, _ in fs], [g_.reshape(-1) for _, _, g_, _ in fs], slot("s0"),
+                                           slot("s1"), lr, b1, b2, eps, [d for _, _, _, d in fs], step,
+                                           masters=slot("master") if extra == "master" else None, los=slot("mlo") if extra == "mlo" else None,
+                                           m_scales=slot("s0_scale"), v_scales=slot("s1_scale"))
 
 
 def common_executables(dims, layouts, kernels, device, hyper) -> dict[str, Any]:

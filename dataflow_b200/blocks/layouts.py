@@ -136,6 +136,12 @@ class DTypePolicy:
             return DTypePolicy(ParamDTypes("bf16", "bf16", "bf16", "lo16"))
         if name == "fp32":
             return DTypePolicy(ParamDTypes("fp32", "fp32", "fp32", None))
+        if name in ("bf16_8bit",):
+            # 8-bit AdamW moments (e4m3 codes, an fp32 scale per 128 elements): half the state of the bf16 policy
+            return DTypePolicy(ParamDTypes("bf16", "bf16", "fp8_e4m3", None))
+        if name in ("bf16_split_master_8bit", "split_master_8bit"):
+            # the exact split master with 8-bit moments: 4 bytes of state per parameter
+            return DTypePolicy(ParamDTypes("bf16", "bf16", "fp8_e4m3", "lo16"))
         if name in ("fp8", "fp8_block"):
             # matrices train through fp8 GEMMs from a bf16 master; everything else stays bf16
             return DTypePolicy(ParamDTypes("bf16", "bf16", "fp32", "fp32"),
@@ -172,7 +178,7 @@ def grad_layout(fields: Sequence[Field], policy: DTypePolicy, layer=None, frozen
 def opt_state_layout(fields: Sequence[Field], policy: DTypePolicy, layer=None,
                      rule_of=lambda f: "adamw") -> PackedLayout:
     """Per field: [``<f>.master`` fp32 | ``<f>.mlo`` int16 low half of a split master] then ``<f>.s0`` … one per
-    optimizer slot."""
+    optimizer slot; an 8-bit slot (``fp8_e4m3``, AdamW only) is followed by its ``<f>.s0_scale``, fp32 per 128 elements."""
     out: list[Field] = []
     for f in fields:
         dt = policy.for_field(f.name, layer)
@@ -183,8 +189,13 @@ def opt_state_layout(fields: Sequence[Field], policy: DTypePolicy, layer=None,
             out.append(Field(f"{f.name}.mlo", f.shape, "int16", f.kind, "zeros"))
         elif dt.master:
             out.append(Field(f"{f.name}.master", f.shape, dt.master, f.kind, "copy"))
+        eight = dt.opt.startswith("fp8")
+        if eight and (rule != "adamw" or dt.opt != "fp8_e4m3"):
+            raise ValueError(f"optimizer state in {dt.opt} exists for AdamW in fp8_e4m3 only (field {f.name!r}, rule {rule!r})")
         for s in range(OPT_SLOTS[rule]):
             out.append(Field(f"{f.name}.s{s}", f.shape, dt.opt, f.kind, "zeros"))
+            if eight:
+                out.append(Field(f"{f.name}.s{s}_scale", ((f.numel + 127) // 128,), "fp32", f.kind, "zeros"))
     return PackedLayout(tuple(out))
 
 

@@ -61,8 +61,35 @@ class _LinearFp8(torch.autograd.Function):
         return dy @ w.t(), x.t() @ dy
 
 
+class _LinearMxfp4(torch.autograd.Function):
+    """y = x @ w with both operands rounded to the microscaled 4-bit format along the contraction in the forward (see ``ops``
+    ``lowbit.linear_fwd_mxfp4``); the backward passes the rounding straight through, on the unquantised operands."""
+
+    @staticmethod
+    def forward(ctx, x, w):
+        from ..ops import resolve_kernels
+        ks = _native(x) or resolve_kernels(kernel_set="eager")
+        ctx.save_for_backward(x, w)
+        return ks.lowbit.linear_fwd_mxfp4(x.contiguous(), w.contiguous())
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w = ctx.saved_tensors
+        need_x, need_w = ctx.needs_input_grad
+        ks = _native(dy) if w.shape[1] % 8 == 0 and dy.shape[0] else None
+        if ks is None:
+            return dy @ w.t() if need_x else None, x.t() @ dy if need_w else None
+        x, w, dy = x.contiguous(), w.contiguous(), dy.contiguous()
+        dw = ks.linear_wgrad_bf16(x, dy, torch.empty_like(w)) if need_w else None
+        return ks.linear_dgrad_bf16(dy, w) if need_x else None, dw
+
+
 def linear(x, w, precision: str = "bf16"):
-    """x (n, k) @ w (k, m); ``precision="fp8"``: e4m3 operands in the forward (see ``ops`` ``linear_fwd_fp8``)."""
+    """x (n, k) @ w (k, m); ``precision="fp8"``: e4m3 operands in the forward (see ``ops`` ``linear_fwd_fp8``); ``"mxfp4"``:
+    4-bit operands.  A contraction length the format does not take (fp8: 16s, mxfp4: 32s) falls back to the plain product."""
+    if precision == "mxfp4" and x.dim() == 2 and x.shape[1] % 32 == 0:
+        return _LinearMxfp4.apply(x, w)
     if precision == "fp8" and x.dim() == 2 and x.shape[1] % 16 == 0 and w.shape[1] % 16 == 0:
         return _LinearFp8.apply(x, w)
     return x @ w

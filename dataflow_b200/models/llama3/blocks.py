@@ -17,12 +17,30 @@ from ...blocks.base_blocks import _Base, common_executables
 # --------------------------------------------------------------------------- stages
 def _lin(K, st):
     """The forward linear of the four large dense projections: bf16, or e4m3 operands with fp32 accumulation when the
-    training configuration asks for ``linear_precision: fp8`` (backward GEMMs stay bf16; router logits stay bf16)."""
+    training configuration asks for ``linear_precision: fp8``, or 4-bit operands for ``mxfp4`` (backward GEMMs stay bf16;
+    router logits stay bf16)."""
+    if st.get("mxfp4"):
+        return lambda x, w, out=None, add=None: _lin_mxfp4(K, x, w, out, add)
     return K.linear_fwd_fp8 if st.get("fp8") else K.linear_fwd_bf16
 
 
+def _lin_mxfp4(K, x, w, out, add):
+    """x is a matrix, or the (codes, scales) that the norm in front of the projection already left."""
+    if not isinstance(x, tuple):
+        return K.lowbit.linear_fwd_mxfp4(x, w, out=out, add=add)
+    return K.lowbit.linear_mxfp4(*x, *K.lowbit.quant_mxfp4(w, transpose=True), out=out, add=add)
+
+
+def _norm_for_lin(K, d, st, x, gain):
+    """The normalised operand of a projection and the row statistics: under ``mxfp4`` the norm writes the 4-bit operand itself."""
+    if st.get("mxfp4"):
+        q, s, _, rstd = K.lowbit.rmsnorm_mxfp4(x, gain, d.eps)
+        return (q, s), rstd
+    return K.rmsnorm_fwd(x, gain, d.eps)
+
+
 def stage_attn_norm(K, d, st):
-    st["h"], rstd = K.rmsnorm_fwd(st["x"], st["w"]["attn_norm"], d.eps)
+    st["h"], rstd = _norm_for_lin(K, d, st, st["x"], st["w"]["attn_norm"])
     st["a"]["rstd_attn"].copy_(rstd)
 
 
@@ -70,7 +88,9 @@ def stage_attn(K, d, st):
 def stage_resid1_norm2(K, d, st):
     h_mid = st["a"]["h_mid"]
     _lin(K, st)(st["a"]["attn_out"], st["w"]["wo"], out=h_mid, add=st["x"])
-    st["h2"], rstd = K.rmsnorm_fwd(h_mid, st["w"]["ffn_norm"], d.eps)
+    # the router of a mixture-of-experts MLP reads the normalised rows in bf16
+    norm = K.rmsnorm_fwd if getattr(d, "moe", False) else lambda x, g, eps: _norm_for_lin(K, d, st, x, g)
+    st["h2"], rstd = norm(h_mid, st["w"]["ffn_norm"], d.eps)
     st["a"]["rstd_ffn"].copy_(rstd)
 
 
@@ -243,7 +263,8 @@ class _Block(_Base):
         seg = self.segments(ctx)
         n = seg.n_tokens
         st = {"seg": seg, "n": n, "x": self.tview(x_buf, (d.T, d.d))[:n], "w": self.views(w_buf, self.lay.block_w),
-              "fp8": self.hyper.get("linear_precision", "bf16") == "fp8"}
+              "fp8": self.hyper.get("linear_precision", "bf16") == "fp8",
+              "mxfp4": self.hyper.get("linear_precision", "bf16") == "mxfp4"}
         if getattr(d, "ep", 1) > 1:
             if n != d.T:
                 raise ValueError("expert-parallel blocks need full rounds (the peers pull exactly T rows from each rank)")
@@ -295,7 +316,10 @@ class BlockRecompute(_Block):
             saved = self.partial_views(ctx.inputs[2], st["n"])
             for name, t in saved.items():
                 st["a"][name].copy_(t)
-            st["h2"] = self.K.rmsnorm_apply(st["a"]["h_mid"], st["w"]["ffn_norm"], st["a"]["rstd_ffn"])
+            if st["mxfp4"] and not self.dims.moe:       # the forward's codes again: same rows, same statistics
+                st["h2"] = self.K.lowbit.rmsnorm_mxfp4(st["a"]["h_mid"], st["w"]["ffn_norm"], self.dims.eps, rstd=st["a"]["rstd_ffn"])[:2]
+            else:
+                st["h2"] = self.K.rmsnorm_apply(st["a"]["h_mid"], st["w"]["ffn_norm"], st["a"]["rstd_ffn"])
             (stage_moe_up if self.dims.moe else stage_up_proj)(self.K, self.dims, st)      # routing is saved context
             return
         for _, fn, _ in recompute_stages(self.stages):

@@ -266,6 +266,7 @@ static void gemm_bf16(const Tensor& A, bool a_mn, const Tensor& B, bool b_mn, Te
     ld_add = addend->stride(0);
   }
   if (bias.has_value()) { CHECK_BF16(*bias); TORCH_CHECK(bias->numel() == N, "bias length mismatch"); }
+  dfb::ensure_context();
   int rc = dfb::gemm_bf16(A.data_ptr(), A.stride(0), a_mn, B.data_ptr(), B.stride(0), b_mn, D.data_ptr(), D.stride(0), d32,
                           optp(addend), ld_add, a32, optp(bias), M, N, K, num_sms(), cur_stream());
   TORCH_CHECK(rc == 0, "gemm_bf16 launch failed with code ", rc);
@@ -672,7 +673,10 @@ static Tensor tensor_from_ptr(int64_t ptr, std::vector<int64_t> shape, const std
   return at::from_blob(reinterpret_cast<void*>(ptr), shape, [](void*) {}, opts);
 }
 
+void bind_lowbit(pybind11::module& m);      // bindings_lowbit.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  bind_lowbit(m);
   m.def("rmsnorm_fwd", &rmsnorm_fwd);
   m.def("rmsnorm_apply", &rmsnorm_apply);
   m.def("rmsnorm_bwd", &rmsnorm_bwd);

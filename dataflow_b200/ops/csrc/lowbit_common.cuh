@@ -1,0 +1,59 @@
+// Device helpers of the narrow formats: e2m1 and e4m3 conversion, e8m0 block scales and their tiled storage.
+#pragma once
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace dfb {
+
+constexpr int kMxBlock = 32;
+constexpr float kE4M3Top = 448.f;
+constexpr float kMinScale = 0x1p-120f;      // floor of an fp32 scale: its reciprocal stays finite
+
+// Byte of (row, block of 32) inside the tiled scales: tiles of 128 rows x 4 blocks, 512 bytes each, `tile_cols` tiles per
+// row of tiles (an even number, so that two tiles = 256 elements of K are one aligned kilobyte).
+DFB_DEVICE long long mx_scale_at(long long row, int block, int tile_cols) {
+  return ((row >> 7) * tile_cols + (block >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
+}
+__host__ __device__ inline int mx_tile_cols(int K) { return 2 * ((K + 255) / 256); }
+
+// Scale byte of a block from its largest magnitude: X = 2^(byte - 127) = 2^max(floor(log2 amax) - 2, -127), so that amax / X is
+// in [4, 8) and saturates at e2m1's 6; 255 (NaN) when the block holds an infinity or a NaN.
+DFB_DEVICE uint32_t mx_scale_byte(float amax) {
+  const uint32_t e = (__float_as_uint(amax) >> 23) & 255u;
+  return e == 255u ? 255u : (e > 2u ? e - 2u : 0u);
+}
+DFB_DEVICE float mx_scale_inv(uint32_t byte) { return __uint_as_float((254u - min(byte, 253u)) << 23); }
+DFB_DEVICE float mx_scale_value(uint32_t byte) {
+  return __uint_as_float(byte == 255u ? 0x7fc00000u : byte == 0u ? 0x00400000u : byte << 23);
+}
+// |x| for a block maximum in which NaN counts as infinity (fmaxf would drop it)
+DFB_DEVICE float mx_abs(float x) { return x == x ? fabsf(x) : INFINITY; }
+
+// eight e2m1 codes, element 0 in the lowest nibble; round to nearest even, saturating
+DFB_DEVICE uint32_t mx_pack8(const float* f) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(r) : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
+  return r;
+}
+// value of a 4-bit code: e2m1 is a half-precision number with 2 exponent bits; built by placing its bits and scaling
+DFB_DEVICE float mx_value(uint32_t code) {
+  const uint32_t mag = code & 7u;
+  const float v = mag < 4u ? 0.5f * mag : (mag < 6u ? mag - 2.f : (mag - 4.f) * 2.f);
+  return (code & 8u) ? -v : v;
+}
+
+// two e4m3 codes: a in the low byte
+DFB_DEVICE uint32_t e4m3_pack2(float a, float b) { return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3); }
+DFB_DEVICE float2 e4m3_unpack2(uint32_t p) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(p), __NV_E4M3);
+  return __half22float2(__half2(h));
+}
+
+}  // namespace dfb

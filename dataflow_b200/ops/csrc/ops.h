@@ -6,6 +6,14 @@
 
 namespace dfb {
 
+// A host thread that has made no runtime call yet (autograd's worker threads) has no current context, and encoding a tensor map
+// fails there.  Setting the thread's own device makes its primary context current; once per thread and device.
+inline void ensure_context() {
+  static thread_local int ready = -1;
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev != ready && cudaSetDevice(dev) == cudaSuccess) ready = dev;
+}
+
 // ---- norms (norm.cu)
 void rmsnorm_fwd(const void* x, const void* w, void* y, float* rstd, int rows, int cols, float eps, cudaStream_t s);
 void rmsnorm_apply(const void* x, const void* w, const float* rstd, void* y, int rows, int cols, cudaStream_t s);

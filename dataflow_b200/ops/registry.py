@@ -47,14 +47,16 @@ class KernelImpl:
 
 
 _REGISTRY: dict[str, list[KernelImpl]] = {}
+# ops of a set other than the core one live in a table of their own and are reached as ``K.<set>.<op>``
+_OP_SETS: dict[str, dict[str, list[KernelImpl]]] = {"core": _REGISTRY, "lowbit": {}}
 
 
 def register(op: str, impl: str, fn: Callable[..., Any] | None = None, *, priority: int = 0,
              requires: Callable[[Mapping[str, Any]], bool] | None = None, deterministic: bool = True,
-             workspace: Workspace | None = None, allocates: bool = False, native: bool = False):
+             workspace: Workspace | None = None, allocates: bool = False, native: bool = False, op_set: str = "core"):
     """Register ``fn`` as implementation ``impl`` of ``op`` (usable as a decorator)."""
     def deco(f):
-        lst = _REGISTRY.setdefault(op, [])
+        lst = _OP_SETS[op_set].setdefault(op, [])
         lst[:] = [k for k in lst if k.name != impl]
         lst.append(KernelImpl(op, impl, f, priority, requires, deterministic,
                               workspace or Workspace.none(), allocates, native))
@@ -62,8 +64,8 @@ def register(op: str, impl: str, fn: Callable[..., Any] | None = None, *, priori
     return deco(fn) if fn is not None else deco
 
 
-def registered_ops() -> dict[str, list[KernelImpl]]:
-    return {k: list(v) for k, v in _REGISTRY.items()}
+def registered_ops(op_set: str = "core") -> dict[str, list[KernelImpl]]:
+    return {k: list(v) for k, v in _OP_SETS[op_set].items()}
 
 
 @dataclass(frozen=True)
@@ -89,13 +91,18 @@ def device_caps(device=None) -> dict[str, Any]:
 
 
 class KernelSet:
-    """Resolved table; ops are attributes: ``K.rmsnorm_fwd(...)``."""
+    """Resolved table; ops are attributes: ``K.rmsnorm_fwd(...)``; the narrow-format ops are ``K.lowbit.quant_mxfp4(...)``."""
 
-    def __init__(self, table: dict[str, KernelImpl], caps: Mapping[str, Any]):
+    def __init__(self, table: dict[str, KernelImpl], caps: Mapping[str, Any], sets: Mapping[str, "KernelSet"] | None = None):
         self._table = dict(table)
         self.caps = dict(caps)
+        self._sets = dict(sets or {})
 
     def __getattr__(self, op: str):
+        if op.startswith("__"):                  # copying and pickling probe for these before the tables exist
+            raise AttributeError(op)
+        if op in self._sets:
+            return self._sets[op]
         try:
             return self._table[op].fn
         except KeyError:
@@ -125,11 +132,18 @@ def resolve_kernels(caps: Mapping[str, Any] | None = None, overrides: Mapping[st
     from . import eager  # noqa: F401  (registers the reference lane)
     from . import library  # noqa: F401
     from . import cuda  # noqa: F401
+    from . import lowbit  # noqa: F401
     caps = dict(caps) if caps is not None else device_caps()
     forced = kernel_set if kernel_set is not None else os.environ.get("DATAFLOW_KERNELS", "")
     overrides = dict(overrides or {})
+    sets = {name: KernelSet(_resolve(ops, caps, overrides, forced), caps) for name, ops in _OP_SETS.items() if name != "core"}
+    return KernelSet(_resolve(_REGISTRY, caps, overrides, forced), caps, sets)
+
+
+def _resolve(registry: Mapping[str, list[KernelImpl]], caps: Mapping[str, Any], overrides: Mapping[str, str],
+             forced: str) -> dict[str, KernelImpl]:
     table: dict[str, KernelImpl] = {}
-    for op, impls in _REGISTRY.items():
+    for op, impls in registry.items():
         usable = [k for k in impls if k.requires is None or k.requires(caps)]
         pick = None
         want = overrides.get(op) or forced
@@ -142,4 +156,4 @@ def resolve_kernels(caps: Mapping[str, Any] | None = None, overrides: Mapping[st
                 continue
             pick = max(usable, key=lambda k: k.priority)
         table[op] = pick
-    return KernelSet(table, caps)
+    return table

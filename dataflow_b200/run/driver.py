@@ -201,6 +201,9 @@ class Trainer:
             if dt.param != "bf16" or dt.grad != "bf16":
                 raise ValueError(f"sharded data parallelism (fsdp / zero*) needs bf16 parameters and gradients (dtype policies bf16, "
                                  f"bf16_master, bf16_split_master); this run asks for {dt.param} / {dt.grad} — use --parallel co for replicas")
+            if dt.opt.startswith("fp8"):
+                raise ValueError("sharded data parallelism (fsdp / zero*) keeps fp32 or bf16 moments per slice: 8-bit optimizer state "
+                                 "(dtype policies *_8bit) runs on one rank or with --parallel co")
         # weights that end a step on the device stay there for the next one (Session.resident)
         self.keep_resident = keep_resident
         # on a device, launch up to two tasks behind an unfinished one: host dispatch hides behind device work

@@ -26,11 +26,11 @@ class Recipe:
     optimizer: str = "adamw"
     muon_lr: float | None = None
     momentum: float = 0.95
-    linear_precision: str = "bf16"      # bf16 | fp8: operand precision of the dense forward projections (llama-like families)
+    linear_precision: str = "bf16"      # bf16 | fp8 | mxfp4: operand precision of the dense forward projections (llama-like families)
 
     def __post_init__(self):
-        if self.linear_precision not in ("bf16", "fp8"):
-            raise ValueError(f"linear_precision must be bf16 or fp8, not {self.linear_precision!r}")
+        if self.linear_precision not in ("bf16", "fp8", "mxfp4"):
+            raise ValueError(f"linear_precision must be bf16, fp8 or mxfp4, not {self.linear_precision!r}")
 
     def lr_schedule(self) -> LRSchedule:
         return LRSchedule(self.schedule, self.peak_lr, self.min_lr, self.warmup_steps, self.total_steps, self.decay_steps)

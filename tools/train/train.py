@@ -35,8 +35,9 @@ def add_run_flags(ap: argparse.ArgumentParser) -> None:
     ap.add_argument("--max-seq-len", type=int, default=None)
     ap.add_argument("--layers", type=int, default=None)
     ap.add_argument("--dtype-policy", default=None)
-    ap.add_argument("--linear-precision", default=None, choices=["bf16", "fp8"],
-                    help="operand precision of the dense forward projections (fp8: e4m3 with per-row / per-column scales)")
+    ap.add_argument("--linear-precision", default=None, choices=["bf16", "fp8", "mxfp4"],
+                    help="operand precision of the dense forward projections (fp8: e4m3 with per-row / per-column scales; mxfp4: 4 bits with a "
+                         "power-of-two scale per 32 elements)")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--fast-budget", type=float, default=None, help="device memory budget in GiB")
     ap.add_argument("--gpus", type=int, default=1)
