@@ -159,7 +159,7 @@ def product_bound(A, B, K, out):
 @pytest.mark.parametrize("dev", LANES)
 @pytest.mark.parametrize("out", [BF, F32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("M,N,K", [(1, 1, 32), (1, 8, 64), (3, 7, 96), (128, 128, 256), (129, 257, 288), (17, 520, 1056), (300, 40, 544),
-                                   (257, 264, 2048), (130, 72, 32), (640, 513, 160)])
+                                   (257, 264, 2048), (130, 72, 32), (640, 513, 160), (2309, 4104, 96)])
 def test_product(dev, out, M, N, K):
     k = lane(dev)
     x = rnd(dev, M, K, seed=M, dtype=F32) * torch.exp(rnd(dev, M, 1, seed=2, dtype=F32))
