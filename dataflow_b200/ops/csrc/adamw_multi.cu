@@ -41,11 +41,14 @@ DFB_DEVICE uint32_t mix32(uint32_t x) {
 
 // e4m3-representable neighbour of y (|y| <= 448) below or above it in magnitude, with the odds of the distance: 16 random bits
 // are added below the kept mantissa and the rest is cut off; adding 2^-6 first puts subnormal codes on one binade's grid.
+// The result may exceed 448 by nothing (448's kept bits are its own, and the conversion saturates); the minimum keeps a NaN's
+// bits from carrying into the sign.
+template <bool SIGNED>
 DFB_DEVICE float dither_e4m3(float y, uint32_t rnd16) {
-  const float a = fabsf(y);
+  const float a = SIGNED ? fabsf(y) : y;
   const float base = a < 0x1p-6f ? 0x1p-6f : 0.f;
-  const float t = __uint_as_float((__float_as_uint(a + base) + (rnd16 << 4)) & 0xfff00000u) - base;
-  return a == a ? copysignf(fminf(t, kE4M3Top), y) : y;        // the bits of a NaN would carry into its sign
+  const float t = __uint_as_float((min(__float_as_uint(a + base), 0x7ff00000u) + (rnd16 << 4)) & 0xfff00000u) - base;
+  return SIGNED ? copysignf(t, y) : t;
 }
 
 template <typename T>
@@ -175,9 +178,9 @@ __global__ void __launch_bounds__(kThreads) adamw_multi_kernel(const __grid_cons
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const uint32_t rnd = mix32((static_cast<uint32_t>(i) + k) * 0x9e3779b9u + salt);
-        qm[k] = dither_e4m3(__fmul_rn(m[k], im), rnd & 0xffffu);
+        qm[k] = dither_e4m3<true>(__fmul_rn(m[k], im), rnd & 0xffffu);
         const float y = __fmul_rn(r[k], ir);
-        qr[k] = dither_e4m3(y, rnd >> 16);
+        qr[k] = dither_e4m3<false>(y, rnd >> 16);
         if (y > 0.f) qr[k] = fmaxf(qr[k], 0x1p-9f);
       }
       store_codes(reinterpret_cast<uint8_t*>(t.m), i, n, vec, qm);
@@ -196,7 +199,7 @@ __global__ void __launch_bounds__(kThreads) adamw_multi_kernel(const __grid_cons
       for (int k = 0; k < 8; ++k) r[k] = sqrtf(r[k]);
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) w[k] -= h.lr * (m[k] * h.inv_bc1 / (r[k] * h.inv_sqrt_bc2 + h.eps) + t.wd * w[k]);
+    for (int k = 0; k < 8; ++k) w[k] -= h.lr * (__fdividef(m[k] * h.inv_bc1, r[k] * h.inv_sqrt_bc2 + h.eps) + t.wd * w[k]);
     if constexpr (WK == kAdamF32) {
       store8(reinterpret_cast<float*>(t.w), i, n, vec, w);
     } else if constexpr (WK == kAdamSplit) {

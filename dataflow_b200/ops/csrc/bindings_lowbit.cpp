@@ -63,7 +63,7 @@ int64_t row_pitch(const char* op, const char* name, const Tensor& t, int64_t col
 int64_t tile_cols(int64_t K) { return 2 * ((K + 255) / 256); }
 void check_mx(const char* op, const char* what, const Tensor& q, const Tensor& s) {
   REFUSE_UNLESS(q.dim() == 2 && q.scalar_type() == at::kByte && q.is_contiguous(), op, ": ", what, "codes are a contiguous (rows, K / 2) uint8 matrix");
-  REFUSE_UNLESS(q.size(1) > 0 && q.size(1) % 16 == 0 && q.size(1) <= 0x3fffffff, op, ": ", what, "codes cover a positive multiple of 32 elements per row");
+  REFUSE_UNLESS(q.size(1) > 0 && q.size(1) % 16 == 0 && q.size(1) <= 65535 * 128, op, ": ", what, "codes cover a positive multiple of 32 elements per row");
   REFUSE_UNLESS(s.scalar_type() == at::kByte && s.is_contiguous() && s.dim() == 3 && s.size(0) == (q.size(0) + 127) / 128 &&
                     s.size(1) == tile_cols(2 * q.size(1)) && s.size(2) == 512,
                 op, ": ", what, "scales are a contiguous uint8 tensor of shape (ceil(rows / 128), 2 ceil(K / 256), 512)");
@@ -79,7 +79,7 @@ std::tuple<Tensor, Tensor> quant_mxfp4(const Tensor& x, bool transpose) {
                 "quant_mxfp4: the last axis of x must be contiguous (transpose=True takes a weight as it is stored)");
   const int64_t rows = transpose ? x.size(1) : x.size(0), K = transpose ? x.size(0) : x.size(1);
   REFUSE_UNLESS(K > 0 && K % 32 == 0, "quant_mxfp4: the contraction length must be a positive multiple of 32");
-  REFUSE_UNLESS(K <= 0x7fffffff - 256, "quant_mxfp4: the contraction is too long");
+  REFUSE_UNLESS(K <= 65535 * 256, "quant_mxfp4: the contraction is too long (at most 16776960)");
   const int64_t ld = x.size(0) > 1 ? x.stride(0) : x.size(1);
   REFUSE_UNLESS(ld >= x.size(1), "quant_mxfp4: rows of x must not overlap");
   on_device("quant_mxfp4", {&x});

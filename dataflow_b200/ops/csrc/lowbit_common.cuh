@@ -42,11 +42,22 @@ DFB_DEVICE uint32_t mx_pack8(const float* f) {
       : "=r"(r) : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
   return r;
 }
-// value of a 4-bit code: e2m1 is a half-precision number with 2 exponent bits; built by placing its bits and scaling
-DFB_DEVICE float mx_value(uint32_t code) {
-  const uint32_t mag = code & 7u;
-  const float v = mag < 4u ? 0.5f * mag : (mag < 6u ? mag - 2.f : (mag - 4.f) * 2.f);
-  return (code & 8u) ? -v : v;
+// the values of eight codes
+DFB_DEVICE void mx_unpack8(uint32_t c, float* f) {
+  uint32_t h[4];
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(c));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+    f[2 * i] = v.x;
+    f[2 * i + 1] = v.y;
+  }
 }
 
 // two e4m3 codes: a in the low byte

@@ -11,55 +11,124 @@ namespace {
 DFB_DEVICE float to_float(float x) { return x; }
 DFB_DEVICE float to_float(bf16 x) { return bf2f(x); }
 
-// one thread per (row, block of 32), the padding of the scale tiles included
-template <typename T, bool TRANS>
-__global__ void __launch_bounds__(256) quant_mxfp4_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q,
-                                                           uint8_t* __restrict__ tiles, long long rows, int K) {
-  const int tile_cols = mx_tile_cols(K), blocks = tile_cols * 4;
-  const long long rows_pad = (rows + 127) / 128 * 128;
-  const long long idx = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
-  // neighbouring threads: neighbouring blocks of a row, or neighbouring rows of a transposed matrix
-  const long long row = TRANS ? idx % rows_pad : idx / blocks;
-  const int b = static_cast<int>(TRANS ? idx / rows_pad : idx % blocks);
-  if (row >= rows_pad || b >= blocks) return;
-  uint32_t sb = 0;
-  if (row < rows && b < K / kMxBlock) {
-    float f[32], amax = 0.f;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const long long k = b * 32 + i;
-      f[i] = to_float(TRANS ? x[k * ldx + row] : x[row * ldx + k]);
-      amax = fmaxf(amax, mx_abs(f[i]));
+template <typename T>
+DFB_DEVICE void load8(const T* p, int live, bool vec, float* f) {      // elements past `live` read as zero
+  if (vec && live >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    } else {
+      unpack8(ld8(p), f);
     }
-    sb = mx_scale_byte(amax);
-    const float inv = mx_scale_inv(sb);
+  } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) f[i] *= inv;
-    *reinterpret_cast<uint4*>(q + row * (K >> 1) + b * 16) = make_uint4(mx_pack8(f), mx_pack8(f + 8), mx_pack8(f + 16), mx_pack8(f + 24));
+    for (int i = 0; i < 8; ++i) f[i] = i < live ? to_float(p[i]) : 0.f;
   }
-  tiles[mx_scale_at(row, b, tile_cols)] = static_cast<uint8_t>(sb);
 }
 
-// one thread per eight elements
+// Along the rows: eight elements per lane, four lanes per block of 32; a warp takes 256 elements of kUnroll rows, all loads in
+// flight at once.  The grid covers the padded scale tiles (whole 128 rows x 256 elements).
+constexpr int kUnroll = 4;
+template <typename T>
+__global__ void __launch_bounds__(256) quant_mxfp4_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q,
+                                                           uint8_t* __restrict__ tiles, long long rows, int K, bool vec) {
+  const int tile_cols = mx_tile_cols(K), k = blockIdx.y * 256 + (threadIdx.x & 31) * 8;
+  const long long row0 = blockIdx.x * (8LL * kUnroll) + (threadIdx.x >> 5) * kUnroll;
+  float f[kUnroll][8];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u)
+    load8(x + (row0 + u) * ldx + k, row0 + u < rows ? K - k : 0, vec, f[u]);       // K - k: a multiple of 8, or not positive
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const long long row = row0 + u;
+    const bool on = row < rows && k < K;
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, mx_abs(f[u][i]));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const uint32_t sb = mx_scale_byte(amax);
+    const float inv = mx_scale_inv(sb);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[u][i] *= inv;
+    if (on) *reinterpret_cast<uint32_t*>(q + row * (K >> 1) + (k >> 1)) = mx_pack8(f[u]);
+    if ((threadIdx.x & 3) == 0) tiles[mx_scale_at(row, k >> 5, tile_cols)] = static_cast<uint8_t>(sb);
+  }
+}
+
+// Along the columns (x stored (K, rows)): a block takes 64 rows x 256 elements of K, warp w the 32 elements of block w.  A lane
+// reads 8 neighbouring rows' values of 8 consecutive k, so that it ends with one whole word of codes per row; the words turn
+// around in shared memory and leave as 128-byte rows.
+template <typename T>
+__global__ void __launch_bounds__(256) quant_mxfp4_cols_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q,
+                                                                uint8_t* __restrict__ tiles, long long rows, int K, bool vec) {
+  __shared__ uint32_t codes[64][33];           // 33: the eight row groups of a store fall on different banks
+  __shared__ uint8_t scales[64][8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = lane & 7, sub = lane >> 3;
+  const int tile_cols = mx_tile_cols(K), k0 = blockIdx.y * 256, kb = k0 + warp * 32 + sub * 8;
+  const long long n0 = blockIdx.x * 64LL, n = n0 + grp * 8;
+  const int live = kb < K ? static_cast<int>(rows - n < 8 ? (rows > n ? rows - n : 0) : 8) : 0;
+  float f[8][8];                               // [k][row]
+#pragma unroll
+  for (int k = 0; k < 8; ++k) load8(x + (kb + k) * ldx + n, live, vec, f[k]);
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    float amax = 0.f, g[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      g[k] = f[k][r];
+      amax = fmaxf(amax, mx_abs(g[k]));
+    }
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 8));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 16));
+    const uint32_t sb = mx_scale_byte(amax);
+    const float inv = mx_scale_inv(sb);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) g[k] *= inv;
+    codes[grp * 8 + r][warp * 4 + sub] = mx_pack8(g);
+    if (sub == 0) scales[grp * 8 + r][warp] = static_cast<uint8_t>(sb);
+  }
+  __syncthreads();
+  for (int r = warp; r < 64; r += 8)
+    if (n0 + r < rows && k0 + lane * 8 < K) *reinterpret_cast<uint32_t*>(q + (n0 + r) * (K >> 1) + (k0 >> 1) + lane * 4) = codes[r][lane];
+  if (threadIdx.x < 128) {                     // four scale bytes of a row are one word of a tile
+    const int r = threadIdx.x >> 1, half = threadIdx.x & 1;
+    *reinterpret_cast<uint32_t*>(tiles + mx_scale_at(n0 + r, (k0 >> 5) + half * 4, tile_cols)) =
+        *reinterpret_cast<const uint32_t*>(&scales[r][half * 4]);
+  }
+}
+
+// The same walk backwards: a warp takes 256 elements of kUnroll rows.
 template <typename T>
 __global__ void __launch_bounds__(256) dequant_mxfp4_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ tiles,
                                                              T* __restrict__ y, long long rows, int K) {
-  const long long idx = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
-  const int nvec = K >> 3;
-  const long long row = idx / nvec;
-  const int v = static_cast<int>(idx % nvec);
-  if (row >= rows) return;
-  const uint32_t c = *reinterpret_cast<const uint32_t*>(q + row * (K >> 1) + v * 4);
-  const float s = mx_scale_value(tiles[mx_scale_at(row, v >> 2, mx_tile_cols(K))]);
-  float f[8];
+  const int tile_cols = mx_tile_cols(K), k = blockIdx.y * 256 + (threadIdx.x & 31) * 8;
+  const long long row0 = blockIdx.x * (8LL * kUnroll) + (threadIdx.x >> 5) * kUnroll;
+  if (k >= K) return;
+  uint32_t c[kUnroll], sb[kUnroll];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = mx_value((c >> (4 * i)) & 15u) * s;
-  T* yp = y + row * K + v * 8;
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(yp) = make_float4(f[0], f[1], f[2], f[3]);
-    *reinterpret_cast<float4*>(yp + 4) = make_float4(f[4], f[5], f[6], f[7]);
-  } else {
-    st8(yp, pack8(f));
+  for (int u = 0; u < kUnroll; ++u) {
+    c[u] = sb[u] = 0;
+    if (row0 + u < rows) {
+      c[u] = *reinterpret_cast<const uint32_t*>(q + (row0 + u) * (K >> 1) + (k >> 1));
+      sb[u] = tiles[mx_scale_at(row0 + u, k >> 5, tile_cols)];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    if (row0 + u >= rows) break;
+    const float s = mx_scale_value(sb[u]);
+    float f[8];
+    mx_unpack8(c[u], f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] *= s;
+    T* yp = y + (row0 + u) * K + k;
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(yp) = make_float4(f[0], f[1], f[2], f[3]);
+      *reinterpret_cast<float4*>(yp + 4) = make_float4(f[4], f[5], f[6], f[7]);
+    } else {
+      st8(yp, pack8(f));
+    }
   }
 }
 
@@ -67,25 +136,31 @@ __global__ void __launch_bounds__(256) dequant_mxfp4_kernel(const uint8_t* __res
 
 int quant_mxfp4(const void* x, long long ldx, int x_f32, int transposed, void* q, void* tiles, long long rows, int K, cudaStream_t s) {
   if (!rows) return 0;
-  const long long n = (rows + 127) / 128 * 128 * mx_tile_cols(K) * 4, grid = (n + 255) / 256;
-  if (grid > 0x7fffffffLL) return -3;
-  auto go = [&](auto kernel, auto* p) { kernel<<<static_cast<unsigned>(grid), 256, 0, s>>>(p, ldx, (uint8_t*)q, (uint8_t*)tiles, rows, K); };
+  const int es = x_f32 ? 4 : 2, segs = mx_tile_cols(K) / 2;
+  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * es) % 16 == 0;       // every row starts on 16 bytes
+  const long long rows_pad = (rows + 127) / 128 * 128;
+  const long long gx = rows_pad / (transposed ? 64 : 8 * kUnroll);
+  if (gx > 0x7fffffffLL || segs > 65535) return -3;
+  const dim3 grid(static_cast<unsigned>(gx), segs);
+  auto go = [&](auto kernel, auto* p) { kernel<<<grid, 256, 0, s>>>(p, ldx, (uint8_t*)q, (uint8_t*)tiles, rows, K, vec); };
   if (x_f32) {
-    if (transposed) go(quant_mxfp4_kernel<float, true>, (const float*)x);
-    else go(quant_mxfp4_kernel<float, false>, (const float*)x);
+    if (transposed) go(quant_mxfp4_cols_kernel<float>, (const float*)x);
+    else go(quant_mxfp4_kernel<float>, (const float*)x);
   } else {
-    if (transposed) go(quant_mxfp4_kernel<bf16, true>, (const bf16*)x);
-    else go(quant_mxfp4_kernel<bf16, false>, (const bf16*)x);
+    if (transposed) go(quant_mxfp4_cols_kernel<bf16>, (const bf16*)x);
+    else go(quant_mxfp4_kernel<bf16>, (const bf16*)x);
   }
   return cudaGetLastError() == cudaSuccess ? 0 : -1;
 }
 
 int dequant_mxfp4(const void* q, const void* tiles, void* y, int y_f32, long long rows, int K, cudaStream_t s) {
-  const long long n = rows * (K >> 3), grid = (n + 255) / 256;
-  if (!n) return 0;
-  if (grid > 0x7fffffffLL) return -3;
-  if (y_f32) dequant_mxfp4_kernel<float><<<static_cast<unsigned>(grid), 256, 0, s>>>((const uint8_t*)q, (const uint8_t*)tiles, (float*)y, rows, K);
-  else dequant_mxfp4_kernel<bf16><<<static_cast<unsigned>(grid), 256, 0, s>>>((const uint8_t*)q, (const uint8_t*)tiles, (bf16*)y, rows, K);
+  if (!rows) return 0;
+  const long long gx = (rows + 8 * kUnroll - 1) / (8 * kUnroll);
+  const int segs = mx_tile_cols(K) / 2;
+  if (gx > 0x7fffffffLL || segs > 65535) return -3;
+  const dim3 grid(static_cast<unsigned>(gx), segs);
+  if (y_f32) dequant_mxfp4_kernel<float><<<grid, 256, 0, s>>>((const uint8_t*)q, (const uint8_t*)tiles, (float*)y, rows, K);
+  else dequant_mxfp4_kernel<bf16><<<grid, 256, 0, s>>>((const uint8_t*)q, (const uint8_t*)tiles, (bf16*)y, rows, K);
   return cudaGetLastError() == cudaSuccess ? 0 : -1;
 }
 

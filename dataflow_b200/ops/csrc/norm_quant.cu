@@ -4,112 +4,234 @@
 //   fp8:    s = max(amax |y| / 448, 2^-120) per row (1 for a row of zeros), q = e4m3(y (1 / s))
 //   mxfp4:  blocks of 32 columns, X = 2^(floor(log2 amax) - 2), q = e2m1(y / X)
 //
-// The statistics are those of the rounded h, the tensor that the backward pass reads again.  One block per row.
+// The statistics are those of the rounded h, the tensor that the backward pass reads again.  Bound by memory: a
+// row is read once into registers (up to 16384 columns) and stays there through both reductions.
 #include "lowbit.h"
 #include "lowbit_common.cuh"
 
 namespace dfb {
 namespace {
 
-template <bool MX, bool RES>
-__global__ void __launch_bounds__(256) rmsnorm_quant_kernel(const bf16* x, long long ldx, const bf16* res, long long ldr,
-                                                             const bf16* __restrict__ w, const float* __restrict__ rstd_in, float eps, bf16* h,
-                                                             long long ldh, uint8_t* __restrict__ q, float* __restrict__ scale,
-                                                             uint8_t* __restrict__ tiles, float* __restrict__ rstd_out, long long rows, int cols) {
-  __shared__ float scratch[33];
-  const long long row = blockIdx.x;
-  const int nvec = cols >> 3;
-  const int tile_cols = mx_tile_cols(cols);
-  if (MX) {
-    // scale bytes past the rows and blocks are zero
-    for (int b = threadIdx.x; b < tile_cols * 4; b += blockDim.x)
-      if (row >= rows || b >= cols / kMxBlock) tiles[mx_scale_at(row, b, tile_cols)] = 0;
-    if (row >= rows) return;
-  }
-  const bf16* xr = x + row * ldx;
-  const bf16* hr = RES ? h + row * ldh : xr;
-  float ss = 0.f;
-  if (RES || !rstd_in) {
-    for (int v = threadIdx.x; v < nvec; v += blockDim.x) {
-      float f[8];
-      unpack8(ld8(xr + v * 8), f);
-      if (RES) {
-        float g[8];
-        unpack8(ld8(res + row * ldr + v * 8), g);
+// max / sum over the T threads of a row; every thread gets the result.  `part` holds one value per warp of the row and is
+// written once per kernel, so a single barrier is enough.
+template <int T, bool MAX>
+DFB_DEVICE float row_reduce(float v, float* part) {
+  v = MAX ? warp_max(v) : warp_sum(v);
+  if constexpr (T > 32) {
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = part[0];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] += g[i];
-        const bf16x8 p = pack8(f);
-        st8(h + row * ldh + v * 8, p);
-        unpack8(p, f);
+    for (int i = 1; i < T / 32; ++i) v = MAX ? fmaxf(v, part[i]) : v + part[i];
+  }
+  return v;
+}
+
+// scale bytes past the rows and past the blocks are zero
+DFB_DEVICE void zero_scale_tail(uint8_t* tiles, long long row, bool dead, int blocks, int tile_cols, int tid, int threads) {
+  for (int b = (dead ? 0 : blocks) + tid; b < tile_cols * 4; b += threads) tiles[mx_scale_at(row, b, tile_cols)] = 0;
+}
+
+DFB_DEVICE void add_round(bf16x8& a, const bf16x8& b) {
+  float f[8], g[8];
+  unpack8(a, f);
+  unpack8(b, g);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] += g[i];
+  a = pack8(f);
+}
+DFB_DEVICE void scaled(const bf16x8& h, const bf16x8& w, float r, float* f) {
+  float g[8];
+  unpack8(h, f);
+  unpack8(w, g);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = f[i] * r * g[i];
+}
+// eight columns of y into the output format; `on` = these columns exist.  mxfp4: four neighbouring lanes hold a block.
+template <bool MX>
+DFB_DEVICE void emit(float* f, float inv, bool on, uint8_t* q, uint8_t* tiles, long long row, int v, int cols, int tile_cols) {
+  if constexpr (MX) {
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, mx_abs(f[i]));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const uint32_t sb = mx_scale_byte(amax);
+    const float iv = mx_scale_inv(sb);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] *= iv;
+    if (on) {
+      *reinterpret_cast<uint32_t*>(q + row * (cols >> 1) + v * 4) = mx_pack8(f);
+      if ((v & 3) == 0) tiles[mx_scale_at(row, v >> 2, tile_cols)] = static_cast<uint8_t>(sb);
+    }
+  } else if (on) {
+    uint2 p;
+    p.x = e4m3_pack2(f[0] * inv, f[1] * inv) | e4m3_pack2(f[2] * inv, f[3] * inv) << 16;
+    p.y = e4m3_pack2(f[4] * inv, f[5] * inv) | e4m3_pack2(f[6] * inv, f[7] * inv) << 16;
+    *reinterpret_cast<uint2*>(q + row * cols + v * 8) = p;
+  }
+}
+
+struct NormArgs {
+  const bf16* x;
+  const bf16* res;
+  const bf16* w;
+  const float* rstd_in;
+  bf16* h;
+  uint8_t* q;
+  float* scale;
+  uint8_t* tiles;
+  float* rstd_out;
+  long long ldx, ldr, ldh, rows;
+  int cols;
+  float eps;
+};
+
+// T threads hold a row in registers, VPT vectors of eight columns each; a block takes max(1, 128 / T) rows.
+template <bool MX, bool RES, int T, int VPT>
+__global__ void __launch_bounds__(T < 128 ? 128 : T) rmsnorm_quant_kernel(const __grid_constant__ NormArgs a) {
+  __shared__ float part[2][T / 32];
+  constexpr int kRows = T < 128 ? 128 / T : 1;
+  const int tid = threadIdx.x % T, nvec = a.cols >> 3, tile_cols = mx_tile_cols(a.cols);
+  const long long row = blockIdx.x * static_cast<long long>(kRows) + threadIdx.x / T;
+  if (MX) zero_scale_tail(a.tiles, row, row >= a.rows, a.cols / kMxBlock, tile_cols, tid, T);
+  if (row >= a.rows) return;                       // whole warps, and whole blocks where a row needs a barrier
+  bf16x8 h[VPT], w[VPT];
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int v = j * T + tid;
+    h[j] = bf16x8{};
+    if (v < nvec) h[j] = ld8(a.x + row * a.ldx + v * 8);
+  }
+  if (RES) {
+    bf16x8 r[VPT];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int v = j * T + tid;
+      r[j] = bf16x8{};
+      if (v < nvec) r[j] = ld8(a.res + row * a.ldr + v * 8);
+    }
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int v = j * T + tid;
+      add_round(h[j], r[j]);
+      if (v < nvec) st8(a.h + row * a.ldh + v * 8, h[j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int v = j * T + tid;
+    w[j] = bf16x8{};
+    if (v < nvec) w[j] = ld8(a.w + v * 8);
+  }
+  float r;
+  if (a.rstd_in) {
+    r = a.rstd_in[row];
+  } else {
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      float f[8];
+      unpack8(h[j], f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss += f[i] * f[i];
+    }
+    r = rsqrtf(row_reduce<T, false>(ss, part[0]) / a.cols + a.eps);
+    if (tid == 0) a.rstd_out[row] = r;
+  }
+  float inv = 1.f;
+  if (!MX) {
+    float amax = 0.f;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      float f[8];
+      scaled(h[j], w[j], r, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(f[i]));
+    }
+    amax = row_reduce<T, true>(amax, part[1]);
+    const float s = amax > 0.f ? fmaxf(__fmul_rn(amax, 1.f / kE4M3Top), kMinScale) : 1.f;
+    inv = __frcp_rn(s);
+    if (tid == 0) a.scale[row] = s;
+  }
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int v = j * T + tid;
+    float f[8];
+    scaled(h[j], w[j], r, f);
+    emit<MX>(f, inv, v < nvec, a.q, a.tiles, row, v, a.cols, tile_cols);
+  }
+}
+
+// Rows too wide for registers: the sum (or x) is read again from cache.
+template <bool MX, bool RES>
+__global__ void __launch_bounds__(512) rmsnorm_quant_wide_kernel(const __grid_constant__ NormArgs a) {
+  __shared__ float part[2][16];
+  const long long row = blockIdx.x;
+  const int nvec = a.cols >> 3, tile_cols = mx_tile_cols(a.cols);
+  if (MX) zero_scale_tail(a.tiles, row, row >= a.rows, a.cols / kMxBlock, tile_cols, threadIdx.x, 512);
+  if (row >= a.rows) return;
+  const bf16* hr = RES ? a.h + row * a.ldh : a.x + row * a.ldx;
+  float ss = 0.f;
+  if (RES || !a.rstd_in) {
+    for (int v = threadIdx.x; v < nvec; v += 512) {
+      bf16x8 h = ld8(a.x + row * a.ldx + v * 8);
+      if (RES) {
+        add_round(h, ld8(a.res + row * a.ldr + v * 8));
+        st8(a.h + row * a.ldh + v * 8, h);
       }
+      float f[8];
+      unpack8(h, f);
 #pragma unroll
       for (int i = 0; i < 8; ++i) ss += f[i] * f[i];
     }
   }
   float r;
-  if (rstd_in) r = rstd_in[row];
-  else r = rsqrtf(block_sum(ss, scratch) / cols + eps);
-  if (threadIdx.x == 0 && rstd_out) rstd_out[row] = r;
-  float s = 1.f, inv = 1.f;
+  if (a.rstd_in) {
+    r = a.rstd_in[row];
+  } else {
+    r = rsqrtf(row_reduce<512, false>(ss, part[0]) / a.cols + a.eps);
+    if (threadIdx.x == 0) a.rstd_out[row] = r;
+  }
+  float inv = 1.f;
   if (!MX) {
     float amax = 0.f;
-    for (int v = threadIdx.x; v < nvec; v += blockDim.x) {
-      float f[8], g[8];
-      unpack8(ld8(hr + v * 8), f);
-      unpack8(ld8(w + v * 8), g);
+    for (int v = threadIdx.x; v < nvec; v += 512) {
+      float f[8];
+      scaled(ld8(hr + v * 8), ld8(a.w + v * 8), r, f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(f[i] * r * g[i]));
+      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(f[i]));
     }
-    amax = block_max(amax, scratch);
-    if (amax > 0.f) s = fmaxf(__fmul_rn(amax, 1.f / kE4M3Top), kMinScale);
+    amax = row_reduce<512, true>(amax, part[1]);
+    const float s = amax > 0.f ? fmaxf(__fmul_rn(amax, 1.f / kE4M3Top), kMinScale) : 1.f;
     inv = __frcp_rn(s);
-    if (threadIdx.x == 0) scale[row] = s;
+    if (threadIdx.x == 0) a.scale[row] = s;
   }
-  for (int v0 = 0; v0 < nvec; v0 += blockDim.x) {
+  for (int v0 = 0; v0 < nvec; v0 += 512) {
     const int v = v0 + threadIdx.x;
-    const bool on = v < nvec;
-    float f[8] = {}, g[8];
-    if (on) {
-      unpack8(ld8(hr + v * 8), f);
-      unpack8(ld8(w + v * 8), g);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = f[i] * r * g[i];
-    }
-    if (MX) {
-      float amax = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, mx_abs(f[i]));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      const uint32_t sb = mx_scale_byte(amax);
-      const float iv = mx_scale_inv(sb);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] *= iv;
-      if (on) {
-        *reinterpret_cast<uint32_t*>(q + row * (cols >> 1) + v * 4) = mx_pack8(f);
-        if ((v & 3) == 0) tiles[mx_scale_at(row, v >> 2, tile_cols)] = static_cast<uint8_t>(sb);
-      }
-    } else if (on) {
-      uint2 p;
-      p.x = e4m3_pack2(f[0] * inv, f[1] * inv) | e4m3_pack2(f[2] * inv, f[3] * inv) << 16;
-      p.y = e4m3_pack2(f[4] * inv, f[5] * inv) | e4m3_pack2(f[6] * inv, f[7] * inv) << 16;
-      *reinterpret_cast<uint2*>(q + row * cols + v * 8) = p;
-    }
+    float f[8] = {};
+    if (v < nvec) scaled(ld8(hr + v * 8), ld8(a.w + v * 8), r, f);
+    emit<MX>(f, inv, v < nvec, a.q, a.tiles, row, v, a.cols, tile_cols);
   }
 }
 
-template <bool MX>
-int launch(const void* x, long long ldx, const void* res, long long ldr, const void* w, const float* rstd_in, float eps, void* h,
-           long long ldh, void* q, float* scale, void* tiles, float* rstd, long long rows, int cols, cudaStream_t s) {
-  if (!rows) return 0;
-  const long long blocks = MX ? (rows + 127) / 128 * 128 : rows;
-  if (blocks > 0x7fffffffLL) return -3;
-  auto go = [&](auto kernel) {
-    kernel<<<static_cast<unsigned>(blocks), 256, 0, s>>>((const bf16*)x, ldx, (const bf16*)res, ldr, (const bf16*)w, rstd_in, eps, (bf16*)h, ldh,
-                                                         (uint8_t*)q, scale, (uint8_t*)tiles, rstd, rows, cols);
+template <bool MX, bool RES>
+int launch(const NormArgs& a, cudaStream_t s) {
+  if (!a.rows) return 0;
+  const long long rows = MX ? (a.rows + 127) / 128 * 128 : a.rows;      // with the padding of the scale tiles
+  if (rows > 0x7fffffffLL) return -3;
+  const int nvec = a.cols >> 3;
+  auto go = [&](auto kernel, int threads, int rows_per_block) {
+    kernel<<<static_cast<unsigned>((rows + rows_per_block - 1) / rows_per_block), threads, 0, s>>>(a);
   };
-  if (res) go(rmsnorm_quant_kernel<MX, true>);
-  else go(rmsnorm_quant_kernel<MX, false>);
+  if (nvec <= 32) go(rmsnorm_quant_kernel<MX, RES, 32, 1>, 128, 4);
+  else if (nvec <= 64) go(rmsnorm_quant_kernel<MX, RES, 32, 2>, 128, 4);
+  else if (nvec <= 128) go(rmsnorm_quant_kernel<MX, RES, 32, 4>, 128, 4);
+  else if (nvec <= 256) go(rmsnorm_quant_kernel<MX, RES, 128, 2>, 128, 1);
+  else if (nvec <= 512) go(rmsnorm_quant_kernel<MX, RES, 128, 4>, 128, 1);
+  else if (nvec <= 1024) go(rmsnorm_quant_kernel<MX, RES, 256, 4>, 256, 1);
+  else if (nvec <= 2048) go(rmsnorm_quant_kernel<MX, RES, 512, 4>, 512, 1);
+  else go(rmsnorm_quant_wide_kernel<MX, RES>, 512, 1);
   return cudaGetLastError() == cudaSuccess ? 0 : -1;
 }
 
@@ -117,11 +239,13 @@ int launch(const void* x, long long ldx, const void* res, long long ldr, const v
 
 int rmsnorm_fp8(const void* x, long long ldx, const void* res, long long ldr, const void* w, const float* rstd_in, float eps, void* h,
                 long long ldh, void* q, float* scale, float* rstd, long long rows, int cols, cudaStream_t s) {
-  return launch<false>(x, ldx, res, ldr, w, rstd_in, eps, h, ldh, q, scale, nullptr, rstd, rows, cols, s);
+  const NormArgs a{(const bf16*)x, (const bf16*)res, (const bf16*)w, rstd_in, (bf16*)h, (uint8_t*)q, scale, nullptr, rstd, ldx, ldr, ldh, rows, cols, eps};
+  return res ? launch<false, true>(a, s) : launch<false, false>(a, s);
 }
 int rmsnorm_mxfp4(const void* x, long long ldx, const void* res, long long ldr, const void* w, const float* rstd_in, float eps, void* h,
                   long long ldh, void* q, void* tiles, float* rstd, long long rows, int cols, cudaStream_t s) {
-  return launch<true>(x, ldx, res, ldr, w, rstd_in, eps, h, ldh, q, nullptr, tiles, rstd, rows, cols, s);
+  const NormArgs a{(const bf16*)x, (const bf16*)res, (const bf16*)w, rstd_in, (bf16*)h, (uint8_t*)q, nullptr, (uint8_t*)tiles, rstd, ldx, ldr, ldh, rows, cols, eps};
+  return res ? launch<true, true>(a, s) : launch<true, false>(a, s);
 }
 
 }  // namespace dfb
