@@ -39,83 +39,92 @@ DFB_DEVICE uint32_t mix32(uint32_t x) {
   return x ^ (x >> 16);
 }
 
-// e4m3-representable neighbour of y (|y| <= 448) below or above it in magnitude, with the odds of the distance: 16 random bits
-// are added below the kept mantissa and the rest is cut off; adding 2^-6 first puts subnormal codes on one binade's grid.
-// The result may exceed 448 by nothing (448's kept bits are its own, and the conversion saturates); the minimum keeps a NaN's
-// bits from carrying into the sign.
-template <bool SIGNED>
-DFB_DEVICE float dither_e4m3(float y, uint32_t rnd16) {
-  const float a = SIGNED ? fabsf(y) : y;
-  const float base = a < 0x1p-6f ? 0x1p-6f : 0.f;
-  const float t = __uint_as_float((min(__float_as_uint(a + base), 0x7ff00000u) + (rnd16 << 4)) & 0xfff00000u) - base;
-  return SIGNED ? copysignf(t, y) : t;
+// Two fp32 operations in one instruction, each rounded to nearest like its scalar form.
+DFB_DEVICE unsigned long long as_u64(float2 a) { return *reinterpret_cast<unsigned long long*>(&a); }
+DFB_DEVICE float2 as_f2(unsigned long long a) { return *reinterpret_cast<float2*>(&a); }
+DFB_DEVICE float2 both(float a) { return make_float2(a, a); }
+DFB_DEVICE float2 mul2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(as_u64(a)), "l"(as_u64(b)));
+  return as_f2(r);
+}
+DFB_DEVICE float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(as_u64(a)), "l"(as_u64(b)), "l"(as_u64(c)));
+  return as_f2(r);
+}
+// within 2^-23 of the root and the reciprocal; numbers below 2^-126 count as zero
+DFB_DEVICE float root(float x) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+DFB_DEVICE float recip(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+DFB_DEVICE float min_nan(float a, float b) {      // the smaller one, or NaN if either is
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
-template <typename T>
-DFB_DEVICE void load8(const T* p, long long i, long long n, bool vec, float* f) {
-  if (vec && i + 8 <= n) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = *reinterpret_cast<const float4*>(p + i), b = *reinterpret_cast<const float4*>(p + i + 4);
-      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-    } else {
-      unpack8(ld8(reinterpret_cast<const bf16*>(p) + i), f);
-    }
+// e4m3-representable neighbour of y (|y| <= 448) below or above it in magnitude, with the odds of the distance: 16 random bits
+// are added below the kept mantissa and the rest is cut off.  448 cannot be left upwards (its kept bits are its own).
+// This form is for 2^-6 <= |y|, where the codes are normal numbers; the sign bit rides along.
+DFB_DEVICE float dither_normal(float y, uint32_t rnd16) { return __uint_as_float((__float_as_uint(y) + (rnd16 << 4)) & 0xfff00000u); }
+// Any y: adding 2^-6 first puts subnormal codes on one binade's grid; the minimum keeps a NaN's bits from carrying.
+DFB_DEVICE float dither_any(float y, uint32_t rnd16) {
+  const float a = fabsf(y);
+  const float base = a < 0x1p-6f ? 0x1p-6f : 0.f;
+  const float t = __uint_as_float((min(__float_as_uint(a + base), 0x7ff00000u) + (rnd16 << 4)) & 0xfff00000u) - base;
+  return copysignf(t, y);
+}
+
+// Eight elements as they lie in memory; a load that may not be whole (FULL false) goes element by element, zeros past n.  The two
+// forms are chosen once per block, so that a thread's loads stand one behind the other without a branch between.
+template <int BYTES>
+struct alignas(BYTES >= 2 ? 16 : 8) Raw { uint32_t u[2 * BYTES]; };      // 8 elements of BYTES bytes
+template <int BYTES, bool FULL>
+DFB_DEVICE Raw<BYTES> load(const void* p, long long i, long long n) {
+  Raw<BYTES> r;
+  if constexpr (FULL) {
+    r = *reinterpret_cast<const Raw<BYTES>*>(static_cast<const char*>(p) + i * BYTES);
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      f[k] = 0.f;
-      if (i + k < n) {
-        if constexpr (sizeof(T) == 4) f[k] = p[i + k];
-        else f[k] = bf2f(p[i + k]);
-      }
-    }
-  }
-}
-template <typename T>
-DFB_DEVICE void store8(T* p, long long i, long long n, bool vec, const float* f) {
-  if (vec && i + 8 <= n) {
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(p + i) = make_float4(f[0], f[1], f[2], f[3]);
-      *reinterpret_cast<float4*>(p + i + 4) = make_float4(f[4], f[5], f[6], f[7]);
-    } else {
-      st8(reinterpret_cast<bf16*>(p) + i, pack8(f));
-    }
-  } else {
+    for (int k = 0; k < 2 * BYTES; ++k) r.u[k] = 0;
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       if (i + k < n) {
-        if constexpr (sizeof(T) == 4) p[i + k] = f[k];
-        else p[i + k] = f2bf(f[k]);
+        if constexpr (BYTES == 4) r.u[k] = static_cast<const uint32_t*>(p)[i + k];
+        else if constexpr (BYTES == 2) r.u[k >> 1] |= static_cast<uint32_t>(static_cast<const uint16_t*>(p)[i + k]) << (16 * (k & 1));
+        else r.u[k >> 2] |= static_cast<uint32_t>(static_cast<const uint8_t*>(p)[i + k]) << (8 * (k & 3));
+      }
+  }
+  return r;
+}
+template <int BYTES, bool FULL>
+DFB_DEVICE void store(void* p, long long i, long long n, const Raw<BYTES>& r) {
+  if constexpr (FULL) {
+    *reinterpret_cast<Raw<BYTES>*>(static_cast<char*>(p) + i * BYTES) = r;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (i + k < n) {
+        if constexpr (BYTES == 4) static_cast<uint32_t*>(p)[i + k] = r.u[k];
+        else if constexpr (BYTES == 2) static_cast<uint16_t*>(p)[i + k] = static_cast<uint16_t>(r.u[k >> 1] >> (16 * (k & 1)));
+        else static_cast<uint8_t*>(p)[i + k] = static_cast<uint8_t>(r.u[k >> 2] >> (8 * (k & 3)));
       }
   }
 }
-DFB_DEVICE void load_codes(const uint8_t* p, long long i, long long n, bool vec, float scale, float* f) {
-  uint2 q = make_uint2(0, 0);
-  if (vec && i + 8 <= n) {
-    q = *reinterpret_cast<const uint2*>(p + i);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (i + k < n) (k < 4 ? q.x : q.y) |= static_cast<uint32_t>(p[i + k]) << (8 * (k & 3));
-  }
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float2 v = e4m3_unpack2(((k < 2 ? q.x : q.y) >> (16 * (k & 1))) & 0xffffu);
-    f[2 * k] = __fmul_rn(v.x, scale);
-    f[2 * k + 1] = __fmul_rn(v.y, scale);
-  }
-}
-DFB_DEVICE void store_codes(uint8_t* p, long long i, long long n, bool vec, const float* f) {
-  uint2 q;
-  q.x = e4m3_pack2(f[0], f[1]) | e4m3_pack2(f[2], f[3]) << 16;
-  q.y = e4m3_pack2(f[4], f[5]) | e4m3_pack2(f[6], f[7]) << 16;
-  if (vec && i + 8 <= n) {
-    *reinterpret_cast<uint2*>(p + i) = q;
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (i + k < n) p[i + k] = static_cast<uint8_t>((k < 4 ? q.x : q.y) >> (8 * (k & 3)));
-  }
+DFB_DEVICE float2 pair(const Raw<4>& r, int j) { return make_float2(__uint_as_float(r.u[2 * j]), __uint_as_float(r.u[2 * j + 1])); }
+DFB_DEVICE float2 pair(const Raw<2>& r, int j) { return make_float2(__uint_as_float(r.u[j] << 16), __uint_as_float(r.u[j] & 0xffff0000u)); }
+DFB_DEVICE float2 pair(const Raw<1>& r, int j) { return e4m3_unpack2((r.u[j >> 1] >> (16 * (j & 1))) & 0xffffu); }
+DFB_DEVICE void set_pair(Raw<4>& r, int j, float2 v) { r.u[2 * j] = __float_as_uint(v.x); r.u[2 * j + 1] = __float_as_uint(v.y); }
+DFB_DEVICE void set_pair(Raw<2>& r, int j, float2 v) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(v.x, v.y);
+  r.u[j] = *reinterpret_cast<const uint32_t*>(&b);
 }
 DFB_DEVICE float max16(float v) {
 #pragma unroll
@@ -123,10 +132,162 @@ DFB_DEVICE float max16(float v) {
   return v;
 }
 
-// The products and sums in front of the stochastic rounding are kept unfused (__fmul_rn, __fadd_rn): a state then has the same
-// code on every machine and in the plain-torch lane.
-template <int WK, typename G, bool BITS8, int NT>
-__global__ void __launch_bounds__(kThreads) adamw_multi_kernel(const __grid_constant__ Args<NT> a) {
+template <int WK, int GB, bool BITS8>
+struct Loaded {
+  Raw<WK == kAdamF32 || WK == kAdamMaster ? 4 : 2> w;
+  Raw<2> lo;                               // split master only
+  Raw<GB> g;
+  Raw<BITS8 ? 1 : 4> m, v;
+  float sm, sv;
+};
+
+// Eight elements of one thread.
+template <int WK, int GB, bool BITS8, bool FULL>
+DFB_DEVICE void step8(const AdamTensor& t, const AdamHyper& h, Loaded<WK, GB, BITS8>& in, long long i) {
+  const long long n = t.n;
+  float2 w[4], m[4], r[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    w[j] = pair(in.w, j);
+    if constexpr (WK == kAdamSplit) {
+      w[j].x = __uint_as_float(__float_as_uint(w[j].x) + static_cast<int32_t>(static_cast<int16_t>(in.lo.u[j] & 0xffffu)));
+      w[j].y = __uint_as_float(__float_as_uint(w[j].y) + static_cast<int32_t>(static_cast<int16_t>(in.lo.u[j] >> 16)));
+    }
+  }
+  const float2 b1 = both(h.b1), c1 = both(h.c1), b2 = both(h.b2), c2 = both(h.c2), gs = both(h.gscale);
+  if constexpr (BITS8) {
+    float am = 0.f, ar = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 g = mul2(pair(in.g, j), gs), r0 = mul2(pair(in.v, j), both(in.sv));
+      m[j] = fma2(mul2(pair(in.m, j), both(in.sm)), b1, mul2(g, c1));
+      const float2 v = fma2(mul2(r0, r0), b2, mul2(mul2(g, g), c2));
+      r[j] = make_float2(root(v.x), root(v.y));
+      am = fmaxf(am, fmaxf(fabsf(m[j].x), fabsf(m[j].y)));
+      ar = fmaxf(ar, fmaxf(r[j].x, r[j].y));
+    }
+    const float sm = fmaxf(__fmul_rn(max16(am), 1.f / kE4M3Top), kMinScale), sr = fmaxf(__fmul_rn(max16(ar), 1.f / kE4M3Top), kMinScale);
+    if ((FULL || i < n) && (threadIdx.x & 15) == 0) {
+      t.m_scale[i >> 7] = sm;
+      t.v_scale[i >> 7] = sr;
+    }
+    const float2 im = both(__frcp_rn(sm)), ir = both(__frcp_rn(sr));
+    float2 y[4], z[4];
+    float low = 0x1p-6f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      y[j] = mul2(m[j], im);
+      z[j] = mul2(r[j], ir);
+      low = min_nan(min_nan(low, min_nan(fabsf(y[j].x), fabsf(y[j].y))), min_nan(z[j].x, z[j].y));
+    }
+    uint32_t x = static_cast<uint32_t>(i) * 0x9e3779b9u + h.seed * 0x85ebca6bu + static_cast<uint32_t>(i >> 32) * 0xc2b2ae35u;
+    // every value of the warp a normal code: almost always, where no moment is zero
+    if (__all_sync(0xffffffffu, low == 0x1p-6f)) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t ra = mix32(x), rb = mix32(x + 0x9e3779b9u);
+        x += 2 * 0x9e3779b9u;
+        y[j] = make_float2(dither_normal(y[j].x, ra & 0xffffu), dither_normal(y[j].y, rb & 0xffffu));
+        z[j] = make_float2(dither_normal(z[j].x, ra >> 16), dither_normal(z[j].y, rb >> 16));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t ra = mix32(x), rb = mix32(x + 0x9e3779b9u);
+        x += 2 * 0x9e3779b9u;
+        y[j] = make_float2(dither_any(y[j].x, ra & 0xffffu), dither_any(y[j].y, rb & 0xffffu));
+        const float2 q = make_float2(dither_any(z[j].x, ra >> 16), dither_any(z[j].y, rb >> 16));
+        // a root above zero keeps at least the smallest code
+        z[j] = make_float2(z[j].x > 0.f ? fmaxf(q.x, 0x1p-9f) : q.x, z[j].y > 0.f ? fmaxf(q.y, 0x1p-9f) : q.y);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      in.m.u[k] = e4m3_pack2(y[2 * k].x, y[2 * k].y) | e4m3_pack2(y[2 * k + 1].x, y[2 * k + 1].y) << 16;
+      in.v.u[k] = e4m3_pack2(z[2 * k].x, z[2 * k].y) | e4m3_pack2(z[2 * k + 1].x, z[2 * k + 1].y) << 16;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 g = mul2(pair(in.g, j), gs);
+      m[j] = fma2(pair(in.m, j), b1, mul2(g, c1));
+      r[j] = fma2(pair(in.v, j), b2, mul2(mul2(g, g), c2));
+      set_pair(in.m, j, m[j]);
+      set_pair(in.v, j, r[j]);
+      r[j] = make_float2(sqrtf(r[j].x), sqrtf(r[j].y));
+    }
+  }
+  store<BITS8 ? 1 : 4, FULL>(t.m, i, n, in.m);
+  store<BITS8 ? 1 : 4, FULL>(t.v, i, n, in.v);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 den = fma2(r[j], both(h.inv_sqrt_bc2), both(h.eps));
+    const float2 up = mul2(mul2(m[j], both(h.inv_bc1)), make_float2(recip(den.x), recip(den.y)));
+    w[j] = fma2(both(-h.lr), fma2(both(t.wd), w[j], up), w[j]);
+  }
+  if constexpr (WK == kAdamSplit) {
+    // the working weight is the master rounded half away from zero, which makes the cut an exact inverse of the join
+    Raw<2> hi;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t a = __float_as_uint(w[j].x), b = __float_as_uint(w[j].y);
+      hi.u[j] = ((a + 0x8000u) >> 16) | ((b + 0x8000u) & 0xffff0000u);
+      in.lo.u[j] = (a & 0xffffu) | (b << 16);
+    }
+    store<2, FULL>(t.w, i, n, hi);
+    store<2, FULL>(t.extra, i, n, in.lo);
+  } else if constexpr (WK == kAdamF32) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) set_pair(in.w, j, w[j]);
+    store<4, FULL>(t.w, i, n, in.w);
+  } else {
+    Raw<2> out;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) set_pair(out, j, w[j]);
+    store<2, FULL>(t.w, i, n, out);
+    if constexpr (WK == kAdamMaster) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) set_pair(in.w, j, w[j]);
+      store<4, FULL>(t.extra, i, n, in.w);
+    }
+  }
+}
+
+// A chunk of one tensor.  With 8-bit moments the loads of both of a thread's groups are issued before the first is computed on.
+template <int WK, int GB, bool BITS8, bool FULL>
+DFB_DEVICE void chunk(const AdamTensor& t, const AdamHyper& h, long long base) {
+  constexpr int kGroups = kChunk / (kThreads * 8), kAhead = BITS8 && FULL ? kGroups : 1;
+  constexpr int WB = WK == kAdamF32 || WK == kAdamMaster ? 4 : 2, SB = BITS8 ? 1 : 4;
+  const long long n = t.n;
+#pragma unroll 1
+  for (int it = 0; it < kGroups; it += kAhead) {
+    Loaded<WK, GB, BITS8> in[kAhead];
+    const long long i0 = base + (it * kThreads + threadIdx.x) * 8LL;
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const long long i = i0 + a * kThreads * 8LL;
+      in[a].w = load<WB, FULL>(WK == kAdamMaster ? t.extra : t.w, i, n);
+      if constexpr (WK == kAdamSplit) in[a].lo = load<2, FULL>(t.extra, i, n);
+      in[a].g = load<GB, FULL>(t.g, i, n);
+      in[a].m = load<SB, FULL>(t.m, i, n);
+      in[a].v = load<SB, FULL>(t.v, i, n);
+      if constexpr (BITS8) {
+        in[a].sm = FULL || i < n ? t.m_scale[i >> 7] : 0.f;
+        in[a].sv = FULL || i < n ? t.v_scale[i >> 7] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      // uniform over the block: the shuffles stay whole.  The scales of a block of 128 are read and written by one half warp, in
+      // that order (the shuffles stand between).
+      if (!FULL && base + (it + a) * kThreads * 8LL >= n) return;
+      step8<WK, GB, BITS8, FULL>(t, h, in[a], i0 + a * kThreads * 8LL);
+    }
+  }
+}
+
+template <int WK, int GB, bool BITS8, int NT>
+__global__ void __launch_bounds__(kThreads, BITS8 ? 3 : 4) adamw_multi_kernel(const __grid_constant__ Args<NT> a) {
   int lo = 0, hi = a.count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -134,88 +295,11 @@ __global__ void __launch_bounds__(kThreads) adamw_multi_kernel(const __grid_cons
     else hi = mid - 1;
   }
   const AdamTensor& t = a.e[lo].t;
-  const AdamHyper& h = a.h;
-  const long long n = t.n, base = static_cast<long long>(blockIdx.x - a.e[lo].first_block) * kChunk;
+  const long long base = static_cast<long long>(blockIdx.x - a.e[lo].first_block) * kChunk;
   const bool vec = ((reinterpret_cast<uintptr_t>(t.w) | reinterpret_cast<uintptr_t>(t.g) | reinterpret_cast<uintptr_t>(t.extra)) & 15) == 0 &&
                    ((reinterpret_cast<uintptr_t>(t.m) | reinterpret_cast<uintptr_t>(t.v)) & (BITS8 ? 7 : 15)) == 0;
-#pragma unroll 1
-  for (int it = 0; it < kChunk / (kThreads * 8); ++it) {
-    const long long i = base + (it * kThreads + threadIdx.x) * 8LL;
-    if (base + it * kThreads * 8LL >= n) break;                    // uniform over the block: the shuffles below stay whole
-    float g[8], m[8], r[8], w[8];
-    load8(reinterpret_cast<const G*>(t.g), i, n, vec, g);
-    if constexpr (WK == kAdamF32) load8(reinterpret_cast<const float*>(t.w), i, n, vec, w);
-    else if constexpr (WK == kAdamMaster) load8(reinterpret_cast<const float*>(t.extra), i, n, vec, w);
-    else load8(reinterpret_cast<const bf16*>(t.w), i, n, vec, w);
-    if constexpr (WK == kAdamSplit) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (i + k < n) w[k] = __uint_as_float(__float_as_uint(w[k]) + static_cast<int32_t>(reinterpret_cast<const int16_t*>(t.extra)[i + k]));
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) g[k] = __fmul_rn(g[k], h.gscale);
-    if constexpr (BITS8) {
-      const bool live = i < n;
-      load_codes(reinterpret_cast<const uint8_t*>(t.m), i, n, vec, live ? t.m_scale[i >> 7] : 0.f, m);
-      load_codes(reinterpret_cast<const uint8_t*>(t.v), i, n, vec, live ? t.v_scale[i >> 7] : 0.f, r);
-      __syncwarp();                                                 // every lane has read its old scale
-      float am = 0.f, ar = 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        m[k] = __fadd_rn(__fmul_rn(m[k], h.b1), __fmul_rn(g[k], h.c1));
-        r[k] = __fsqrt_rn(__fadd_rn(__fmul_rn(__fmul_rn(r[k], r[k]), h.b2), __fmul_rn(__fmul_rn(g[k], g[k]), h.c2)));
-        am = fmaxf(am, fabsf(m[k]));
-        ar = fmaxf(ar, r[k]);
-      }
-      const float sm = fmaxf(__fmul_rn(max16(am), 1.f / kE4M3Top), kMinScale), sr = fmaxf(__fmul_rn(max16(ar), 1.f / kE4M3Top), kMinScale);
-      if (live && (threadIdx.x & 15) == 0) {
-        t.m_scale[i >> 7] = sm;
-        t.v_scale[i >> 7] = sr;
-      }
-      const float im = __frcp_rn(sm), ir = __frcp_rn(sr);
-      float qm[8], qr[8];
-      const uint32_t salt = h.seed * 0x85ebca6bu + static_cast<uint32_t>(i >> 32) * 0xc2b2ae35u;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t rnd = mix32((static_cast<uint32_t>(i) + k) * 0x9e3779b9u + salt);
-        qm[k] = dither_e4m3<true>(__fmul_rn(m[k], im), rnd & 0xffffu);
-        const float y = __fmul_rn(r[k], ir);
-        qr[k] = dither_e4m3<false>(y, rnd >> 16);
-        if (y > 0.f) qr[k] = fmaxf(qr[k], 0x1p-9f);
-      }
-      store_codes(reinterpret_cast<uint8_t*>(t.m), i, n, vec, qm);
-      store_codes(reinterpret_cast<uint8_t*>(t.v), i, n, vec, qr);
-    } else {
-      load8(reinterpret_cast<const float*>(t.m), i, n, vec, m);
-      load8(reinterpret_cast<const float*>(t.v), i, n, vec, r);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        m[k] = m[k] * h.b1 + g[k] * h.c1;
-        r[k] = r[k] * h.b2 + g[k] * g[k] * h.c2;
-      }
-      store8(reinterpret_cast<float*>(t.m), i, n, vec, m);
-      store8(reinterpret_cast<float*>(t.v), i, n, vec, r);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) r[k] = sqrtf(r[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) w[k] -= h.lr * (__fdividef(m[k] * h.inv_bc1, r[k] * h.inv_sqrt_bc2 + h.eps) + t.wd * w[k]);
-    if constexpr (WK == kAdamF32) {
-      store8(reinterpret_cast<float*>(t.w), i, n, vec, w);
-    } else if constexpr (WK == kAdamSplit) {
-      // the working weight is the master rounded half away from zero, which makes the cut an exact inverse of the join
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (i + k < n) {
-          const uint32_t b = __float_as_uint(w[k]);
-          reinterpret_cast<uint16_t*>(t.w)[i + k] = static_cast<uint16_t>((b + 0x8000u) >> 16);
-          reinterpret_cast<uint16_t*>(t.extra)[i + k] = static_cast<uint16_t>(b);
-        }
-    } else {
-      if constexpr (WK == kAdamMaster) store8(reinterpret_cast<float*>(t.extra), i, n, vec, w);
-      store8(reinterpret_cast<bf16*>(t.w), i, n, vec, w);
-    }
-  }
+  if (vec && base + kChunk <= t.n) chunk<WK, GB, BITS8, true>(t, a.h, base);
+  else chunk<WK, GB, BITS8, false>(t, a.h, base);
 }
 
 template <int NT>
@@ -231,15 +315,10 @@ int launch(const AdamTensor* t, int count, int weights, bool g_f32, bool bits8, 
   a.count = count;
   a.h = h;
   auto go = [&](auto kernel) { kernel<<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(a); };
-  auto by_bits = [&](auto wk, auto gt) {
-    constexpr int WK = decltype(wk)::value;
-    using G = decltype(gt);
-    if (bits8) go(adamw_multi_kernel<WK, G, true, NT>);
-    else go(adamw_multi_kernel<WK, G, false, NT>);
-  };
   auto by_grad = [&](auto wk) {
-    if (g_f32) by_bits(wk, float{});
-    else by_bits(wk, bf16{});
+    constexpr int WK = decltype(wk)::value;
+    if (g_f32) bits8 ? go(adamw_multi_kernel<WK, 4, true, NT>) : go(adamw_multi_kernel<WK, 4, false, NT>);
+    else bits8 ? go(adamw_multi_kernel<WK, 2, true, NT>) : go(adamw_multi_kernel<WK, 2, false, NT>);
   };
   switch (weights) {
     case kAdamBf16: by_grad(std::integral_constant<int, kAdamBf16>{}); break;
@@ -255,7 +334,9 @@ int launch(const AdamTensor* t, int count, int weights, bool g_f32, bool bits8, 
 
 // ``t`` holds no empty tensor.  A list longer than the table goes out in several launches.
 int adamw_multi(const AdamTensor* t, int count, int weights, bool g_f32, bool bits8, const AdamHyper& h, cudaStream_t s) {
-  constexpr int kMany = 256;
+  // a table of 256 is 20 KB of kernel parameters, one of 24 is 2 KB: a layer's fields fit the small one
+  constexpr int kFew = 24, kMany = 256;
+  if (count <= kFew) return launch<kFew>(t, count, weights, g_f32, bits8, h, s);
   for (int at = 0; at < count; at += kMany) {
     const int rc = launch<kMany>(t + at, count - at < kMany ? count - at : kMany, weights, g_f32, bits8, h, s);
     if (rc) return rc;

@@ -60,6 +60,13 @@ DFB_DEVICE void mx_unpack8(uint32_t c, float* f) {
   }
 }
 
+// Scale bytes of four neighbouring blocks (lanes 0-3, 4-7, 8-11, 12-15 of a half warp hold one each) as the tile's word.
+DFB_DEVICE uint32_t mx_scale_word(uint32_t byte) {
+  uint32_t w = byte << (8 * ((threadIdx.x >> 2) & 3));
+  w |= __shfl_xor_sync(0xffffffffu, w, 4);
+  return w | __shfl_xor_sync(0xffffffffu, w, 8);
+}
+
 // two e4m3 codes: a in the low byte
 DFB_DEVICE uint32_t e4m3_pack2(float a, float b) { return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3); }
 DFB_DEVICE float2 e4m3_unpack2(uint32_t p) {

@@ -8,69 +8,95 @@
 namespace dfb {
 namespace {
 
-DFB_DEVICE float to_float(float x) { return x; }
-DFB_DEVICE float to_float(bf16 x) { return bf2f(x); }
-
+// Eight elements as they lie in memory.  A load that may not be whole (FULL false) goes element by element, zeros past `live`;
+// the two forms are chosen once per block, so that a whole block's loads stand one behind the other without a branch between.
 template <typename T>
-DFB_DEVICE void load8(const T* p, int live, bool vec, float* f) {      // elements past `live` read as zero
-  if (vec && live >= 8) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-    } else {
-      unpack8(ld8(p), f);
-    }
+struct Raw8 { T v[8]; };
+template <>
+struct Raw8<bf16> { bf16x8 v; };
+template <>
+struct Raw8<float> { float4 a, b; };
+template <bool FULL>
+DFB_DEVICE Raw8<bf16> load8(const bf16* p, int live) {
+  Raw8<bf16> r;
+  if constexpr (FULL) {
+    r.v = ld8(p);
   } else {
+    bf16* e = reinterpret_cast<bf16*>(&r);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = i < live ? to_float(p[i]) : 0.f;
+    for (int i = 0; i < 8; ++i) e[i] = i < live ? p[i] : f2bf(0.f);
   }
+  return r;
+}
+template <bool FULL>
+DFB_DEVICE Raw8<float> load8(const float* p, int live) {
+  Raw8<float> r;
+  if constexpr (FULL) {
+    r.a = *reinterpret_cast<const float4*>(p);
+    r.b = *reinterpret_cast<const float4*>(p + 4);
+  } else {
+    float* e = reinterpret_cast<float*>(&r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = i < live ? p[i] : 0.f;
+  }
+  return r;
+}
+DFB_DEVICE void widen(const Raw8<bf16>& r, float* f) { unpack8(r.v, f); }
+DFB_DEVICE void widen(const Raw8<float>& r, float* f) {
+  f[0] = r.a.x; f[1] = r.a.y; f[2] = r.a.z; f[3] = r.a.w;
+  f[4] = r.b.x; f[5] = r.b.y; f[6] = r.b.z; f[7] = r.b.w;
 }
 
 // Along the rows: eight elements per lane, four lanes per block of 32; a warp takes 256 elements of kUnroll rows, all loads in
 // flight at once.  The grid covers the padded scale tiles (whole 128 rows x 256 elements).
 constexpr int kUnroll = 4;
-template <typename T>
-__global__ void __launch_bounds__(256) quant_mxfp4_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q,
-                                                           uint8_t* __restrict__ tiles, long long rows, int K, bool vec) {
+template <typename T, bool FULL>
+DFB_DEVICE void quant_rows(const T* x, long long ldx, uint8_t* q, uint8_t* tiles, long long rows, int K) {
   const int tile_cols = mx_tile_cols(K), k = blockIdx.y * 256 + (threadIdx.x & 31) * 8;
   const long long row0 = blockIdx.x * (8LL * kUnroll) + (threadIdx.x >> 5) * kUnroll;
-  float f[kUnroll][8];
+  Raw8<T> raw[kUnroll];
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u)
-    load8(x + (row0 + u) * ldx + k, row0 + u < rows ? K - k : 0, vec, f[u]);       // K - k: a multiple of 8, or not positive
+  for (int u = 0; u < kUnroll; ++u) raw[u] = load8<FULL>(x + (row0 + u) * ldx + k, row0 + u < rows ? K - k : 0);
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     const long long row = row0 + u;
-    const bool on = row < rows && k < K;
-    float amax = 0.f;
+    float f[8], amax = 0.f;
+    widen(raw[u], f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, mx_abs(f[u][i]));
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, mx_abs(f[i]));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
     const uint32_t sb = mx_scale_byte(amax);
     const float inv = mx_scale_inv(sb);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[u][i] *= inv;
-    if (on) *reinterpret_cast<uint32_t*>(q + row * (K >> 1) + (k >> 1)) = mx_pack8(f[u]);
-    if ((threadIdx.x & 3) == 0) tiles[mx_scale_at(row, k >> 5, tile_cols)] = static_cast<uint8_t>(sb);
+    for (int i = 0; i < 8; ++i) f[i] *= inv;
+    if (FULL || (row < rows && k < K)) *reinterpret_cast<uint32_t*>(q + row * (K >> 1) + (k >> 1)) = mx_pack8(f);
+    const uint32_t word = mx_scale_word(sb);
+    if ((threadIdx.x & 15) == 0) *reinterpret_cast<uint32_t*>(tiles + mx_scale_at(row, k >> 5, tile_cols)) = word;
   }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) quant_mxfp4_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q,
+                                                           uint8_t* __restrict__ tiles, long long rows, int K, bool vec) {
+  if (vec && (blockIdx.x + 1) * (8LL * kUnroll) <= rows && static_cast<int>(blockIdx.y + 1) * 256 <= K) quant_rows<T, true>(x, ldx, q, tiles, rows, K);
+  else quant_rows<T, false>(x, ldx, q, tiles, rows, K);
 }
 
 // Along the columns (x stored (K, rows)): a block takes 64 rows x 256 elements of K, warp w the 32 elements of block w.  A lane
 // reads 8 neighbouring rows' values of 8 consecutive k, so that it ends with one whole word of codes per row; the words turn
 // around in shared memory and leave as 128-byte rows.
-template <typename T>
-__global__ void __launch_bounds__(256) quant_mxfp4_cols_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q,
-                                                                uint8_t* __restrict__ tiles, long long rows, int K, bool vec) {
-  __shared__ uint32_t codes[64][33];           // 33: the eight row groups of a store fall on different banks
-  __shared__ uint8_t scales[64][8];
+template <typename T, bool FULL>
+DFB_DEVICE void quant_cols(const T* x, long long ldx, long long rows, int K, uint32_t (*codes)[33], uint8_t (*scales)[8]) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, grp = lane & 7, sub = lane >> 3;
-  const int tile_cols = mx_tile_cols(K), k0 = blockIdx.y * 256, kb = k0 + warp * 32 + sub * 8;
-  const long long n0 = blockIdx.x * 64LL, n = n0 + grp * 8;
+  const int kb = blockIdx.y * 256 + warp * 32 + sub * 8;
+  const long long n = blockIdx.x * 64LL + grp * 8;
   const int live = kb < K ? static_cast<int>(rows - n < 8 ? (rows > n ? rows - n : 0) : 8) : 0;
+  Raw8<T> raw[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) raw[k] = load8<FULL>(x + (kb + k) * ldx + n, live);
   float f[8][8];                               // [k][row]
 #pragma unroll
-  for (int k = 0; k < 8; ++k) load8(x + (kb + k) * ldx + n, live, vec, f[k]);
+  for (int k = 0; k < 8; ++k) widen(raw[k], f[k]);
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
     float amax = 0.f, g[8];
@@ -88,6 +114,16 @@ __global__ void __launch_bounds__(256) quant_mxfp4_cols_kernel(const T* __restri
     codes[grp * 8 + r][warp * 4 + sub] = mx_pack8(g);
     if (sub == 0) scales[grp * 8 + r][warp] = static_cast<uint8_t>(sb);
   }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) quant_mxfp4_cols_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q,
+                                                                uint8_t* __restrict__ tiles, long long rows, int K, bool vec) {
+  __shared__ uint32_t codes[64][33];           // 33: the eight row groups of a store fall on different banks
+  __shared__ __align__(4) uint8_t scales[64][8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tile_cols = mx_tile_cols(K), k0 = blockIdx.y * 256;
+  const long long n0 = blockIdx.x * 64LL;
+  if (vec && n0 + 64 <= rows && k0 + 256 <= K) quant_cols<T, true>(x, ldx, rows, K, codes, scales);
+  else quant_cols<T, false>(x, ldx, rows, K, codes, scales);
   __syncthreads();
   for (int r = warp; r < 64; r += 8)
     if (n0 + r < rows && k0 + lane * 8 < K) *reinterpret_cast<uint32_t*>(q + (n0 + r) * (K >> 1) + (k0 >> 1) + lane * 4) = codes[r][lane];

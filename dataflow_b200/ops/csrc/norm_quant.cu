@@ -27,9 +27,9 @@ DFB_DEVICE float row_reduce(float v, float* part) {
   return v;
 }
 
-// scale bytes past the rows and past the blocks are zero
+// scale bytes past the rows and past the blocks are zero (the last word of a row's own blocks is written whole by emit)
 DFB_DEVICE void zero_scale_tail(uint8_t* tiles, long long row, bool dead, int blocks, int tile_cols, int tid, int threads) {
-  for (int b = (dead ? 0 : blocks) + tid; b < tile_cols * 4; b += threads) tiles[mx_scale_at(row, b, tile_cols)] = 0;
+  for (int b = (dead ? 0 : (blocks + 3) / 4 * 4) + tid; b < tile_cols * 4; b += threads) tiles[mx_scale_at(row, b, tile_cols)] = 0;
 }
 
 DFB_DEVICE void add_round(bf16x8& a, const bf16x8& b) {
@@ -60,9 +60,10 @@ DFB_DEVICE void emit(float* f, float inv, bool on, uint8_t* q, uint8_t* tiles, l
     const float iv = mx_scale_inv(sb);
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] *= iv;
+    const uint32_t word = mx_scale_word(sb);          // columns that do not exist count as zero blocks
     if (on) {
       *reinterpret_cast<uint32_t*>(q + row * (cols >> 1) + v * 4) = mx_pack8(f);
-      if ((v & 3) == 0) tiles[mx_scale_at(row, v >> 2, tile_cols)] = static_cast<uint8_t>(sb);
+      if ((v & 15) == 0) *reinterpret_cast<uint32_t*>(tiles + mx_scale_at(row, v >> 2, tile_cols)) = word;
     }
   } else if (on) {
     uint2 p;
