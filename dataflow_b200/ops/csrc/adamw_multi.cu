@@ -8,7 +8,7 @@
 // index, seed).  A positive r keeps at least the smallest code.  The update itself uses the unrounded moments.
 //
 // The kernel moves 10 bytes per element with 8-bit moments (28 with fp32 moments and a master) and is bound by memory: a block
-// takes 4096 consecutive elements of one tensor, a thread eight at a time, sixteen lanes share one scale.  Tensors travel as a
+// takes 4096 consecutive elements of one tensor, a thread eight or (8-bit moments) sixteen of them, so that eight lanes share a scale.  Tensors travel as a
 // table in the kernel's parameters (no copy, no device-side table that a captured graph would share); a block finds its tensor
 // by bisection.
 #include "lowbit.h"
@@ -17,7 +17,13 @@
 namespace dfb {
 namespace {
 
-constexpr int kChunk = 4096, kThreads = 256;
+constexpr int kChunk = 4096;
+// Threads of a block, and blocks per SM.  The 8-bit form at 176M parameters: sixteen elements a thread, 64 threads, 10 blocks
+// (96 registers) 334 us; 128 threads at 4 / 5 / 6 blocks 355 / 340 / 336 us; eight elements a thread 379 us at best.
+template <bool BITS8>
+constexpr int kThreads = BITS8 ? 64 : 256;
+template <bool BITS8>
+constexpr int kBlocks = BITS8 ? 10 : 4;
 
 struct Entry {
   AdamTensor t;
@@ -39,37 +45,23 @@ DFB_DEVICE uint32_t mix32(uint32_t x) {
   return x ^ (x >> 16);
 }
 
-// Two fp32 operations in one instruction, each rounded to nearest like its scalar form.
-DFB_DEVICE unsigned long long as_u64(float2 a) { return *reinterpret_cast<unsigned long long*>(&a); }
-DFB_DEVICE float2 as_f2(unsigned long long a) { return *reinterpret_cast<float2*>(&a); }
-DFB_DEVICE float2 both(float a) { return make_float2(a, a); }
-DFB_DEVICE float2 mul2(float2 a, float2 b) {
-  unsigned long long r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(as_u64(a)), "l"(as_u64(b)));
-  return as_f2(r);
+// Square roots, rounded to nearest: Heron's step on an approximate reciprocal root with the residual from a fused product
+// (Markstein 1990, "Computation of elementary functions on the IBM RISC System/6000 processor"), checked against sqrtf over
+// whole binades: the same from 2^-90 up, a last place off now and then below 2^-102, 0 for 0).
+DFB_DEVICE float2 root2(float2 x) {
+  float2 y;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(fmaxf(x.x, 0x1p-126f)));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(fmaxf(x.y, 0x1p-126f)));
+  const float2 s = mul2(x, y);
+  const float2 e = fma2(make_float2(-s.x, -s.y), s, x);
+  return fma2(e, mul2(y, both(0.5f)), s);
 }
-DFB_DEVICE float2 fma2(float2 a, float2 b, float2 c) {
-  unsigned long long r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(as_u64(a)), "l"(as_u64(b)), "l"(as_u64(c)));
-  return as_f2(r);
-}
-// within 2^-23 of the root and the reciprocal; numbers below 2^-126 count as zero
-DFB_DEVICE float root(float x) {
-  float r;
-  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
+// within 2^-23 of the reciprocal
 DFB_DEVICE float recip(float x) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-DFB_DEVICE float min_nan(float a, float b) {      // the smaller one, or NaN if either is
-  float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // e4m3-representable neighbour of y (|y| <= 448) below or above it in magnitude, with the odds of the distance: 16 random bits
 // are added below the kept mantissa and the rest is cut off.  448 cannot be left upwards (its kept bits are its own).
 // This form is for 2^-6 <= |y|, where the codes are normal numbers; the sign bit rides along.
@@ -84,18 +76,18 @@ DFB_DEVICE float dither_any(float y, uint32_t rnd16) {
 
 // Eight elements as they lie in memory; a load that may not be whole (FULL false) goes element by element, zeros past n.  The two
 // forms are chosen once per block, so that a thread's loads stand one behind the other without a branch between.
-template <int BYTES>
-struct alignas(BYTES >= 2 ? 16 : 8) Raw { uint32_t u[2 * BYTES]; };      // 8 elements of BYTES bytes
-template <int BYTES, bool FULL>
-DFB_DEVICE Raw<BYTES> load(const void* p, long long i, long long n) {
-  Raw<BYTES> r;
+template <int BYTES, int E>
+struct alignas(BYTES * E >= 16 ? 16 : 8) Raw { uint32_t u[BYTES * E / 4]; };      // E elements of BYTES bytes, 16 bytes at least
+template <int BYTES, int E, bool FULL>
+DFB_DEVICE Raw<BYTES, E> load(const void* p, long long i, long long n) {
+  Raw<BYTES, E> r;
   if constexpr (FULL) {
-    r = *reinterpret_cast<const Raw<BYTES>*>(static_cast<const char*>(p) + i * BYTES);
+    r = *reinterpret_cast<const Raw<BYTES, E>*>(static_cast<const char*>(p) + i * BYTES);
   } else {
 #pragma unroll
-    for (int k = 0; k < 2 * BYTES; ++k) r.u[k] = 0;
+    for (int k = 0; k < BYTES * E / 4; ++k) r.u[k] = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
+    for (int k = 0; k < E; ++k)
       if (i + k < n) {
         if constexpr (BYTES == 4) r.u[k] = static_cast<const uint32_t*>(p)[i + k];
         else if constexpr (BYTES == 2) r.u[k >> 1] |= static_cast<uint32_t>(static_cast<const uint16_t*>(p)[i + k]) << (16 * (k & 1));
@@ -104,13 +96,13 @@ DFB_DEVICE Raw<BYTES> load(const void* p, long long i, long long n) {
   }
   return r;
 }
-template <int BYTES, bool FULL>
-DFB_DEVICE void store(void* p, long long i, long long n, const Raw<BYTES>& r) {
+template <int BYTES, int E, bool FULL>
+DFB_DEVICE void store(void* p, long long i, long long n, const Raw<BYTES, E>& r) {
   if constexpr (FULL) {
-    *reinterpret_cast<Raw<BYTES>*>(static_cast<char*>(p) + i * BYTES) = r;
+    *reinterpret_cast<Raw<BYTES, E>*>(static_cast<char*>(p) + i * BYTES) = r;
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
+    for (int k = 0; k < E; ++k)
       if (i + k < n) {
         if constexpr (BYTES == 4) static_cast<uint32_t*>(p)[i + k] = r.u[k];
         else if constexpr (BYTES == 2) static_cast<uint16_t*>(p)[i + k] = static_cast<uint16_t>(r.u[k >> 1] >> (16 * (k & 1)));
@@ -118,64 +110,78 @@ DFB_DEVICE void store(void* p, long long i, long long n, const Raw<BYTES>& r) {
       }
   }
 }
-DFB_DEVICE float2 pair(const Raw<4>& r, int j) { return make_float2(__uint_as_float(r.u[2 * j]), __uint_as_float(r.u[2 * j + 1])); }
-DFB_DEVICE float2 pair(const Raw<2>& r, int j) { return make_float2(__uint_as_float(r.u[j] << 16), __uint_as_float(r.u[j] & 0xffff0000u)); }
-DFB_DEVICE float2 pair(const Raw<1>& r, int j) { return e4m3_unpack2((r.u[j >> 1] >> (16 * (j & 1))) & 0xffffu); }
-DFB_DEVICE void set_pair(Raw<4>& r, int j, float2 v) { r.u[2 * j] = __float_as_uint(v.x); r.u[2 * j + 1] = __float_as_uint(v.y); }
-DFB_DEVICE void set_pair(Raw<2>& r, int j, float2 v) {
+template <int E>
+DFB_DEVICE float2 pair(const Raw<4, E>& r, int j) { return make_float2(__uint_as_float(r.u[2 * j]), __uint_as_float(r.u[2 * j + 1])); }
+template <int E>
+DFB_DEVICE float2 pair(const Raw<2, E>& r, int j) { return make_float2(__uint_as_float(r.u[j] << 16), __uint_as_float(r.u[j] & 0xffff0000u)); }
+template <int E>
+DFB_DEVICE float2 pair(const Raw<1, E>& r, int j) { return e4m3_unpack2((r.u[j >> 1] >> (16 * (j & 1))) & 0xffffu); }
+template <int E>
+DFB_DEVICE void set_pair(Raw<4, E>& r, int j, float2 v) { r.u[2 * j] = __float_as_uint(v.x); r.u[2 * j + 1] = __float_as_uint(v.y); }
+template <int E>
+DFB_DEVICE void set_pair(Raw<2, E>& r, int j, float2 v) {
   const __nv_bfloat162 b = __floats2bfloat162_rn(v.x, v.y);
   r.u[j] = *reinterpret_cast<const uint32_t*>(&b);
 }
-DFB_DEVICE float max16(float v) {
+// over the lanes that share a scale: 128 elements
+template <int LANES>
+DFB_DEVICE float max_lanes(float v) {
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
 
+// elements per thread: sixteen with 8-bit moments (one 16-byte load of codes, half the shuffles per element), else eight
+template <bool BITS8>
+constexpr int kPer = BITS8 ? 16 : 8;
+
 template <int WK, int GB, bool BITS8>
 struct Loaded {
-  Raw<WK == kAdamF32 || WK == kAdamMaster ? 4 : 2> w;
-  Raw<2> lo;                               // split master only
-  Raw<GB> g;
-  Raw<BITS8 ? 1 : 4> m, v;
+  static constexpr int E = kPer<BITS8>;
+  Raw<WK == kAdamF32 || WK == kAdamMaster ? 4 : 2, E> w;
+  Raw<2, E> lo;                            // split master only
+  Raw<GB, E> g;
+  Raw<BITS8 ? 1 : 4, E> m, v;
   float sm, sv;
 };
 
-// Eight elements of one thread.
+// The elements of one thread.  Products and sums in front of the 8-bit rounding are rounded one by one (a sum is a fused product
+// with a factor of one that the compiler does not know), so a state has the same codes here and in the plain-torch lane.
 template <int WK, int GB, bool BITS8, bool FULL>
-DFB_DEVICE void step8(const AdamTensor& t, const AdamHyper& h, Loaded<WK, GB, BITS8>& in, long long i) {
+DFB_DEVICE void step(const AdamTensor& t, const AdamHyper& h, Loaded<WK, GB, BITS8>& in, long long i) {
+  constexpr int E = kPer<BITS8>, P = E / 2;
   const long long n = t.n;
-  float2 w[4], m[4], r[4];
+  float2 w[P], m[P], r[P];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < P; ++j) {
     w[j] = pair(in.w, j);
     if constexpr (WK == kAdamSplit) {
       w[j].x = __uint_as_float(__float_as_uint(w[j].x) + static_cast<int32_t>(static_cast<int16_t>(in.lo.u[j] & 0xffffu)));
       w[j].y = __uint_as_float(__float_as_uint(w[j].y) + static_cast<int32_t>(static_cast<int16_t>(in.lo.u[j] >> 16)));
     }
   }
+  const float2 one = both(h.one);
   const float2 b1 = both(h.b1), c1 = both(h.c1), b2 = both(h.b2), c2 = both(h.c2), gs = both(h.gscale);
   if constexpr (BITS8) {
     float am = 0.f, ar = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < P; ++j) {
       const float2 g = mul2(pair(in.g, j), gs), r0 = mul2(pair(in.v, j), both(in.sv));
-      m[j] = fma2(mul2(pair(in.m, j), both(in.sm)), b1, mul2(g, c1));
-      const float2 v = fma2(mul2(r0, r0), b2, mul2(mul2(g, g), c2));
-      r[j] = make_float2(root(v.x), root(v.y));
+      m[j] = fma2(mul2(mul2(pair(in.m, j), both(in.sm)), b1), one, mul2(g, c1));
+      r[j] = root2(fma2(mul2(mul2(r0, r0), b2), one, mul2(mul2(g, g), c2)));
       am = fmaxf(am, fmaxf(fabsf(m[j].x), fabsf(m[j].y)));
       ar = fmaxf(ar, fmaxf(r[j].x, r[j].y));
     }
-    const float sm = fmaxf(__fmul_rn(max16(am), 1.f / kE4M3Top), kMinScale), sr = fmaxf(__fmul_rn(max16(ar), 1.f / kE4M3Top), kMinScale);
-    if ((FULL || i < n) && (threadIdx.x & 15) == 0) {
+    const float sm = fmaxf(__fmul_rn(max_lanes<128 / E>(am), 1.f / kE4M3Top), kMinScale), sr = fmaxf(__fmul_rn(max_lanes<128 / E>(ar), 1.f / kE4M3Top), kMinScale);
+    if ((FULL || i < n) && (threadIdx.x & (128 / E - 1)) == 0) {
       t.m_scale[i >> 7] = sm;
       t.v_scale[i >> 7] = sr;
     }
     const float2 im = both(__frcp_rn(sm)), ir = both(__frcp_rn(sr));
-    float2 y[4], z[4];
+    float2 y[P], z[P];
     float low = 0x1p-6f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < P; ++j) {
       y[j] = mul2(m[j], im);
       z[j] = mul2(r[j], ir);
       low = min_nan(min_nan(low, min_nan(fabsf(y[j].x), fabsf(y[j].y))), min_nan(z[j].x, z[j].y));
@@ -184,7 +190,7 @@ DFB_DEVICE void step8(const AdamTensor& t, const AdamHyper& h, Loaded<WK, GB, BI
     // every value of the warp a normal code: almost always, where no moment is zero
     if (__all_sync(0xffffffffu, low == 0x1p-6f)) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < P; ++j) {
         const uint32_t ra = mix32(x), rb = mix32(x + 0x9e3779b9u);
         x += 2 * 0x9e3779b9u;
         y[j] = make_float2(dither_normal(y[j].x, ra & 0xffffu), dither_normal(y[j].y, rb & 0xffffu));
@@ -192,7 +198,7 @@ DFB_DEVICE void step8(const AdamTensor& t, const AdamHyper& h, Loaded<WK, GB, BI
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < P; ++j) {
         const uint32_t ra = mix32(x), rb = mix32(x + 0x9e3779b9u);
         x += 2 * 0x9e3779b9u;
         y[j] = make_float2(dither_any(y[j].x, ra & 0xffffu), dither_any(y[j].y, rb & 0xffffu));
@@ -202,13 +208,13 @@ DFB_DEVICE void step8(const AdamTensor& t, const AdamHyper& h, Loaded<WK, GB, BI
       }
     }
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < E / 4; ++k) {
       in.m.u[k] = e4m3_pack2(y[2 * k].x, y[2 * k].y) | e4m3_pack2(y[2 * k + 1].x, y[2 * k + 1].y) << 16;
       in.v.u[k] = e4m3_pack2(z[2 * k].x, z[2 * k].y) | e4m3_pack2(z[2 * k + 1].x, z[2 * k + 1].y) << 16;
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < P; ++j) {
       const float2 g = mul2(pair(in.g, j), gs);
       m[j] = fma2(pair(in.m, j), b1, mul2(g, c1));
       r[j] = fma2(pair(in.v, j), b2, mul2(mul2(g, g), c2));
@@ -217,77 +223,68 @@ DFB_DEVICE void step8(const AdamTensor& t, const AdamHyper& h, Loaded<WK, GB, BI
       r[j] = make_float2(sqrtf(r[j].x), sqrtf(r[j].y));
     }
   }
-  store<BITS8 ? 1 : 4, FULL>(t.m, i, n, in.m);
-  store<BITS8 ? 1 : 4, FULL>(t.v, i, n, in.v);
+  store<BITS8 ? 1 : 4, E, FULL>(t.m, i, n, in.m);
+  store<BITS8 ? 1 : 4, E, FULL>(t.v, i, n, in.v);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < P; ++j) {
     const float2 den = fma2(r[j], both(h.inv_sqrt_bc2), both(h.eps));
     const float2 up = mul2(mul2(m[j], both(h.inv_bc1)), make_float2(recip(den.x), recip(den.y)));
     w[j] = fma2(both(-h.lr), fma2(both(t.wd), w[j], up), w[j]);
   }
   if constexpr (WK == kAdamSplit) {
     // the working weight is the master rounded half away from zero, which makes the cut an exact inverse of the join
-    Raw<2> hi;
+    Raw<2, E> hi;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < P; ++j) {
       const uint32_t a = __float_as_uint(w[j].x), b = __float_as_uint(w[j].y);
       hi.u[j] = ((a + 0x8000u) >> 16) | ((b + 0x8000u) & 0xffff0000u);
       in.lo.u[j] = (a & 0xffffu) | (b << 16);
     }
-    store<2, FULL>(t.w, i, n, hi);
-    store<2, FULL>(t.extra, i, n, in.lo);
+    store<2, E, FULL>(t.w, i, n, hi);
+    store<2, E, FULL>(t.extra, i, n, in.lo);
   } else if constexpr (WK == kAdamF32) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) set_pair(in.w, j, w[j]);
-    store<4, FULL>(t.w, i, n, in.w);
+    for (int j = 0; j < P; ++j) set_pair(in.w, j, w[j]);
+    store<4, E, FULL>(t.w, i, n, in.w);
   } else {
-    Raw<2> out;
+    Raw<2, E> out;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) set_pair(out, j, w[j]);
-    store<2, FULL>(t.w, i, n, out);
+    for (int j = 0; j < P; ++j) set_pair(out, j, w[j]);
+    store<2, E, FULL>(t.w, i, n, out);
     if constexpr (WK == kAdamMaster) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) set_pair(in.w, j, w[j]);
-      store<4, FULL>(t.extra, i, n, in.w);
+      for (int j = 0; j < P; ++j) set_pair(in.w, j, w[j]);
+      store<4, E, FULL>(t.extra, i, n, in.w);
     }
   }
 }
 
-// A chunk of one tensor.  With 8-bit moments the loads of both of a thread's groups are issued before the first is computed on.
+// A chunk of one tensor.
 template <int WK, int GB, bool BITS8, bool FULL>
 DFB_DEVICE void chunk(const AdamTensor& t, const AdamHyper& h, long long base) {
-  constexpr int kGroups = kChunk / (kThreads * 8), kAhead = BITS8 && FULL ? kGroups : 1;
+  constexpr int E = kPer<BITS8>, kGroups = kChunk / (kThreads<BITS8> * E);
   constexpr int WB = WK == kAdamF32 || WK == kAdamMaster ? 4 : 2, SB = BITS8 ? 1 : 4;
   const long long n = t.n;
 #pragma unroll 1
-  for (int it = 0; it < kGroups; it += kAhead) {
-    Loaded<WK, GB, BITS8> in[kAhead];
-    const long long i0 = base + (it * kThreads + threadIdx.x) * 8LL;
-#pragma unroll
-    for (int a = 0; a < kAhead; ++a) {
-      const long long i = i0 + a * kThreads * 8LL;
-      in[a].w = load<WB, FULL>(WK == kAdamMaster ? t.extra : t.w, i, n);
-      if constexpr (WK == kAdamSplit) in[a].lo = load<2, FULL>(t.extra, i, n);
-      in[a].g = load<GB, FULL>(t.g, i, n);
-      in[a].m = load<SB, FULL>(t.m, i, n);
-      in[a].v = load<SB, FULL>(t.v, i, n);
-      if constexpr (BITS8) {
-        in[a].sm = FULL || i < n ? t.m_scale[i >> 7] : 0.f;
-        in[a].sv = FULL || i < n ? t.v_scale[i >> 7] : 0.f;
-      }
+  for (int it = 0; it < kGroups; ++it) {
+    const long long first = base + it * kThreads<BITS8> * static_cast<long long>(E), i = first + threadIdx.x * E;
+    if (!FULL && first >= n) return;         // uniform over the block: the shuffles stay whole
+    Loaded<WK, GB, BITS8> in;
+    in.w = load<WB, E, FULL>(WK == kAdamMaster ? t.extra : t.w, i, n);
+    if constexpr (WK == kAdamSplit) in.lo = load<2, E, FULL>(t.extra, i, n);
+    in.g = load<GB, E, FULL>(t.g, i, n);
+    in.m = load<SB, E, FULL>(t.m, i, n);
+    in.v = load<SB, E, FULL>(t.v, i, n);
+    if constexpr (BITS8) {                   // read here, written behind the shuffles of the lanes that share it
+      in.sm = FULL || i < n ? t.m_scale[i >> 7] : 0.f;
+      in.sv = FULL || i < n ? t.v_scale[i >> 7] : 0.f;
     }
-#pragma unroll
-    for (int a = 0; a < kAhead; ++a) {
-      // uniform over the block: the shuffles stay whole.  The scales of a block of 128 are read and written by one half warp, in
-      // that order (the shuffles stand between).
-      if (!FULL && base + (it + a) * kThreads * 8LL >= n) return;
-      step8<WK, GB, BITS8, FULL>(t, h, in[a], i0 + a * kThreads * 8LL);
-    }
+    step<WK, GB, BITS8, FULL>(t, h, in, i);
   }
 }
 
 template <int WK, int GB, bool BITS8, int NT>
-__global__ void __launch_bounds__(kThreads, BITS8 ? 3 : 4) adamw_multi_kernel(const __grid_constant__ Args<NT> a) {
+__global__ void __launch_bounds__(kThreads<BITS8>, kBlocks<BITS8>) adamw_multi_kernel(const __grid_constant__ Args<NT> a) {
   int lo = 0, hi = a.count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -297,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, BITS8 ? 3 : 4) adamw_multi_kernel(co
   const AdamTensor& t = a.e[lo].t;
   const long long base = static_cast<long long>(blockIdx.x - a.e[lo].first_block) * kChunk;
   const bool vec = ((reinterpret_cast<uintptr_t>(t.w) | reinterpret_cast<uintptr_t>(t.g) | reinterpret_cast<uintptr_t>(t.extra)) & 15) == 0 &&
-                   ((reinterpret_cast<uintptr_t>(t.m) | reinterpret_cast<uintptr_t>(t.v)) & (BITS8 ? 7 : 15)) == 0;
+                   ((reinterpret_cast<uintptr_t>(t.m) | reinterpret_cast<uintptr_t>(t.v)) & 15) == 0;
   if (vec && base + kChunk <= t.n) chunk<WK, GB, BITS8, true>(t, a.h, base);
   else chunk<WK, GB, BITS8, false>(t, a.h, base);
 }
@@ -314,7 +311,7 @@ int launch(const AdamTensor* t, int count, int weights, bool g_f32, bool bits8, 
   if (blocks > 0x7fffffffLL) return -3;
   a.count = count;
   a.h = h;
-  auto go = [&](auto kernel) { kernel<<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(a); };
+  auto go = [&](auto kernel) { kernel<<<static_cast<unsigned>(blocks), bits8 ? kThreads<true> : kThreads<false>, 0, s>>>(a); };
   auto by_grad = [&](auto wk) {
     constexpr int WK = decltype(wk)::value;
     if (g_f32) bits8 ? go(adamw_multi_kernel<WK, 4, true, NT>) : go(adamw_multi_kernel<WK, 4, false, NT>);

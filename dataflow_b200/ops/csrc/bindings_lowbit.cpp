@@ -182,12 +182,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rmsnorm_narrow(bool mx, const Tensor&
     auto u8 = x.options().dtype(at::kByte);
     Tensor q = at::empty({rows, cols / 2}, u8), s = at::empty({(rows + 127) / 128, tile_cols(cols), 512}, u8);
     launched(dfb::rmsnorm_mxfp4(x.const_data_ptr(), ldx, rp, ldr, w.const_data_ptr(), given, (float)eps, hp, ldh, q.data_ptr(), s.data_ptr(), rstd_out,
-                                rows, (int)cols, stream_of(x)), op);
+                                rows, (int)cols, sms(x), stream_of(x)), op);
     return {q, s, h, rstd};
   }
   Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn)), s = at::empty({rows}, x.options().dtype(at::kFloat));
   launched(dfb::rmsnorm_fp8(x.const_data_ptr(), ldx, rp, ldr, w.const_data_ptr(), given, (float)eps, hp, ldh, q.data_ptr(), s.data_ptr<float>(), rstd_out,
-                            rows, (int)cols, stream_of(x)), op);
+                            rows, (int)cols, sms(x), stream_of(x)), op);
   return {q, s, h, rstd};
 }
 

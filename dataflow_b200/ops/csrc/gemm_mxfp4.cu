@@ -345,6 +345,178 @@ bool make_map(CUtensorMap* m, CUtensorMapDataType type, const void* base, uint64
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+
+// ---------------------------------------------------------------------------------------------------------------------------
+// Few tiles: rows of B (the weight) are the 128 rows of a CTA's MMA, up to 128 rows of A its columns, and the CTAs of a cluster
+// split K.  Each leaves its partial sums in its own shared memory; then every CTA of the cluster adds a share of them up, in rank
+// order (the result does not depend on who came first), and writes it.  A weight of 4096 x 4096 for a few tokens is spread over
+// 128 SMs instead of 32.
+namespace skinny {
+constexpr int TM = 128, TN = 128;                                            // weight rows, tokens
+constexpr int STAGES = 6;
+constexpr int W_BYTES = TM * BK / 2, X_BYTES = TN * BK / 2, SF_BYTES = 2 * SF_TILE;
+constexpr int STAGE_BYTES = W_BYTES + X_BYTES + 2 * SF_BYTES;
+constexpr int SF_COL = 128, SF_STRIDE = 16, TMEM_COLS = 256;
+constexpr int THREADS = 128;
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
+static_assert(STAGES * STAGE_BYTES >= TM * TN * 4, "the partial sums take the stages' place");
+
+struct Barriers {
+  uint64_t full[STAGES], empty[STAGES], done;
+  uint32_t tmem_base;
+  int abort;
+};
+
+DFB_PTX void umma_mxf4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+      : : "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+}
+DFB_PTX void scales_to_tmem(uint32_t taddr, uint32_t smem_addr) {
+  const uint64_t desc = static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4) | (static_cast<uint64_t>(128 >> 4) << 32) | ptx::kDescVersion;
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" : : "r"(taddr), "l"(desc) : "memory");
+}
+DFB_PTX float4 load_remote(uint32_t smem_addr, uint32_t rank) {
+  float4 v;
+  asm volatile(
+      "{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %4, %5;\n\t"
+      "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [ra];\n\t}"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(smem_addr), "r"(rank) : "memory");
+  return v;
+}
+
+// grid (splits * tiles of N, tiles of M), clusters of `splits` along x
+__global__ void __launch_bounds__(THREADS, 1)
+gemm_mxfp4_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
+                         const __grid_constant__ CUtensorMap tmap_sw, const __grid_constant__ CUtensorMap tmap_sx, Params p, int splits) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Barriers* sb = reinterpret_cast<Barriers*>(smem + STAGES * STAGE_BYTES);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(ptx::cluster_ctarank());
+  const int n0 = (blockIdx.x / splits) * TM, m0 = blockIdx.y * TN;
+  const int tokens = min(TN, p.M - m0), mma_n = (tokens + 15) & ~15;
+  const int k_blocks = (p.K + BK - 1) / BK, per = (k_blocks + splits - 1) / splits;
+  const int k_lo = min(rank * per, k_blocks), k_hi = min(k_lo + per, k_blocks);
+  volatile int* abort_flag = &sb->abort;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { ptx::mbar_init(&sb->full[s], 1); ptx::mbar_init(&sb->empty[s], 1); }
+    ptx::mbar_init(&sb->done, 1);
+    sb->abort = 0;
+    ptx::mbar_fence_init();
+    ptx::prefetch_tmap(&tmap_w);
+    ptx::prefetch_tmap(&tmap_x);
+    ptx::prefetch_tmap(&tmap_sw);
+    ptx::prefetch_tmap(&tmap_sx);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(&sb->tmem_base, TMEM_COLS);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = sb->tmem_base;
+  if (warp == 0) {
+    if (ptx::elect_one()) {
+      for (int kb = k_lo, it = 0; kb < k_hi; ++kb, ++it) {
+        const int s = it % STAGES;
+        if (!ptx::mbar_wait(&sb->empty[s], ((it / STAGES) & 1) ^ 1, abort_flag)) { sb->abort = 1; atomicExch(&g_error, 21); break; }
+        uint8_t* st = smem + s * STAGE_BYTES;
+        ptx::mbar_expect_tx(&sb->full[s], STAGE_BYTES);
+        ptx::tma_load_2d(st, &tmap_w, &sb->full[s], kb * (BK / 2), n0);
+        ptx::tma_load_2d(st + W_BYTES, &tmap_x, &sb->full[s], kb * (BK / 2), m0);
+        ptx::tma_load_2d(st + W_BYTES + X_BYTES, &tmap_sw, &sb->full[s], 0, (n0 >> 7) * k_blocks + kb);
+        ptx::tma_load_2d(st + W_BYTES + X_BYTES + SF_BYTES, &tmap_sx, &sb->full[s], 0, (m0 >> 7) * k_blocks + kb);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (ptx::elect_one()) {
+      bool failed = false;
+      for (int kb = k_lo, it = 0; kb < k_hi; ++kb, ++it) {
+        const int s = it % STAGES;
+        if (!ptx::mbar_wait(&sb->full[s], (it / STAGES) & 1, abort_flag)) { sb->abort = 1; atomicExch(&g_error, 22); failed = true; break; }
+        ptx::tc_fence_after();
+        const uint32_t w_addr = ptx::smem_u32(smem + s * STAGE_BYTES), sf = w_addr + W_BYTES + X_BYTES;
+        const uint32_t sfw = tmem_base + SF_COL + (it & 1) * SF_STRIDE, sfx = sfw + 8;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          scales_to_tmem(sfw + c * 4, sf + c * SF_TILE);
+          scales_to_tmem(sfx + c * 4, sf + SF_BYTES + c * SF_TILE);
+        }
+        const uint64_t wdesc = ptx::desc_kmajor_sw128(w_addr), xdesc = ptx::desc_kmajor_sw128(w_addr + W_BYTES);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          umma_mxf4(tmem_base, wdesc + k * 2, xdesc + k * 2, idesc_mxf4(TM, mma_n, k & 1), sfw + (k >> 1) * 4, sfx + (k >> 1) * 4, it != 0 || k != 0);
+        ptx::umma_commit(&sb->empty[s]);
+      }
+      if (!failed) ptx::umma_commit(&sb->done);
+    }
+    __syncwarp();
+  }
+  // partial sums to shared memory, one token's 128 values in a row: every copy into the stages has been read by then
+  float* part = reinterpret_cast<float*>(smem);
+  if (!ptx::mbar_wait(&sb->done, 0, abort_flag)) { sb->abort = 1; atomicExch(&g_error, 23); }
+  ptx::tc_fence_after();
+  const uint32_t taddr = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
+  for (int c = 0; c < tokens; c += 32) {
+    uint32_t r[32];
+    ptx::tmem_ld_32x32(taddr + c, r);
+    ptx::tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (c + i < tokens) part[(c + i) * TM + warp * 32 + lane] = k_lo < k_hi ? __uint_as_float(r[i]) : 0.f;
+  }
+  ptx::tc_fence_before();
+  ptx::cluster_sync();
+  // this CTA's share of the tokens: one warp takes a token, a lane four neighbouring outputs
+  const int n = n0 + lane * 4;
+  for (int t = rank * 4 + warp; t < tokens; t += splits * 4) {
+    const uint32_t at = ptx::smem_u32(part + t * TM + lane * 4);
+    float f[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < splits; ++r) {
+      const float4 v = load_remote(at, r);
+      f[0] += v.x; f[1] += v.y; f[2] += v.z; f[3] += v.w;
+    }
+    const long long row = m0 + t;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < p.N) {
+        if (p.bias) f[i] += bf2f(reinterpret_cast<const bf16*>(p.bias)[n + i]);
+        if (p.d_is_f32) {
+          if (p.addend) f[i] += reinterpret_cast<const float*>(p.addend)[row * p.ld_add + n + i];
+          reinterpret_cast<float*>(p.D)[row * p.ldd + n + i] = f[i];
+        } else {
+          if (p.addend) f[i] += bf2f(reinterpret_cast<const bf16*>(p.addend)[row * p.ld_add + n + i]);
+          reinterpret_cast<bf16*>(p.D)[row * p.ldd + n + i] = f2bf(f[i]);
+        }
+      }
+  }
+  __syncthreads();
+  if (*abort_flag && threadIdx.x == 0) {
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);      // let copies still in flight land
+  }
+  ptx::cluster_sync();                     // nobody leaves while its sums may still be read
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+}  // namespace skinny
+
+// cudaFuncSetAttribute once per kernel and device
+template <typename Kernel>
+bool configure(Kernel kernel, int smem_bytes, std::atomic<bool>* done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return false;
+  if (done[dev].load()) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes) != cudaSuccess) return false;
+  done[dev].store(true);
+  return true;
+}
+
 }  // namespace mx
 }  // namespace
 
@@ -378,19 +550,38 @@ int gemm_mxfp4(const void* A, const void* sa, const void* B, const void* sb, voi
   p.ldd = ldd; p.ld_add = ld_add; p.d_is_f32 = d_f32;
   p.group_m = 16;
   p.tma_epi = tma_epi;
-  static std::atomic<bool> configured[64];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -1;
-  if (!configured[dev].load()) {
-    if (cudaFuncSetAttribute(gemm_mxfp4_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) return -1;
-    configured[dev].store(true);
-  }
+  // The pair kernel takes `waves` rounds of k_blocks stages over the pairs.  Where its tiles leave SMs idle the skinny kernel
+  // may need fewer stages per CTA; a stage costs about the same in both (it is the loads that take the time).
   const int clusters = num_sms / 2;
+  const long long ctas = (N + skinny::TM - 1) / skinny::TM * ((M + skinny::TN - 1) / skinny::TN);
+  int splits = 1;
+  while (splits < 8 && ctas * splits * 2 <= num_sms && splits * 2 <= k_blocks) splits *= 2;
+  const long long pair_cost = (tiles + clusters - 1) / clusters * k_blocks;
+  const long long skinny_cost = (ctas * splits + num_sms - 1) / num_sms * ((k_blocks + splits - 1) / splits);
+  if (skinny_cost < pair_cost && (M + skinny::TN - 1) / skinny::TN <= 65535) {
+    static std::atomic<bool> ready[64];
+    if (!configure(skinny::gemm_mxfp4_skinny_kernel, skinny::SMEM_BYTES, ready)) return -1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>((N + skinny::TM - 1) / skinny::TM) * splits, static_cast<unsigned>((M + skinny::TN - 1) / skinny::TN));
+    cfg.blockDim = dim3(skinny::THREADS);
+    cfg.dynamicSmemBytes = skinny::SMEM_BYTES;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = splits;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, skinny::gemm_mxfp4_skinny_kernel, tb, ta, tsb, tsa, p, splits) == cudaSuccess ? 0 : -1;
+  }
+  static std::atomic<bool> ready[64];
+  if (!configure(gemm_mxfp4_kernel, SMEM_BYTES, ready)) return -1;
   gemm_mxfp4_kernel<<<2 * static_cast<int>(tiles < clusters ? tiles : clusters), THREADS, SMEM_BYTES, stream>>>(ta, tb, tsa, tsb, td, tadd, p);
   return cudaGetLastError() == cudaSuccess ? 0 : -1;
 }
 
-// The kernel's error word on the current device: 0, or which bounded wait ran out (11 producer, 12 / 13 MMA, 14 / 15 epilogue)
+// The kernel's error word on the current device: 0, or which bounded wait ran out (11 producer, 12 / 13 MMA, 14 / 15 epilogue; 21 to 23 the same of
+// the kernel for few tiles)
 int gemm_mxfp4_last_error() {
   int v = 0;
   return cudaMemcpyFromSymbol(&v, mx::g_error, sizeof(int)) == cudaSuccess ? v : -1;

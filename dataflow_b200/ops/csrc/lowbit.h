@@ -22,14 +22,15 @@ enum AdamWeights { kAdamBf16 = 0, kAdamF32 = 1, kAdamMaster = 2, kAdamSplit = 3 
 struct AdamHyper {
   float lr, b1, c1, b2, c2, eps, inv_bc1, inv_sqrt_bc2, gscale;
   uint32_t seed;
+  float one = 1.f;
 };
 int adamw_multi(const AdamTensor* t, int count, int weights, bool g_f32, bool bits8, const AdamHyper& h, cudaStream_t s);
 
 // h = bf16(x + residual) (h == null: x is taken as it is), y = h * rstd * w.  rstd_in: statistics to apply (null: computed).
 int rmsnorm_fp8(const void* x, long long ldx, const void* res, long long ldr, const void* w, const float* rstd_in, float eps, void* h,
-                long long ldh, void* q, float* scale, float* rstd, long long rows, int cols, cudaStream_t s);
+                long long ldh, void* q, float* scale, float* rstd, long long rows, int cols, int num_sms, cudaStream_t s);
 int rmsnorm_mxfp4(const void* x, long long ldx, const void* res, long long ldr, const void* w, const float* rstd_in, float eps, void* h,
-                  long long ldh, void* q, void* tiles, float* rstd, long long rows, int cols, cudaStream_t s);
+                  long long ldh, void* q, void* tiles, float* rstd, long long rows, int cols, int num_sms, cudaStream_t s);
 
 // x (rows, K), row pitch ldx elements (transposed: x (K, rows), pitch of a K row); q (rows, K / 2), tiles as in lowbit_common.cuh
 int quant_mxfp4(const void* x, long long ldx, int x_f32, int transposed, void* q, void* tiles, long long rows, int K, cudaStream_t s);

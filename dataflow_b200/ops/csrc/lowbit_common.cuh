@@ -10,6 +10,32 @@ constexpr int kMxBlock = 32;
 constexpr float kE4M3Top = 448.f;
 constexpr float kMinScale = 0x1p-120f;      // floor of an fp32 scale: its reciprocal stays finite
 
+// Two fp32 operations in one instruction, each rounded to nearest like its scalar form.
+DFB_DEVICE unsigned long long as_u64(float2 a) { return *reinterpret_cast<unsigned long long*>(&a); }
+DFB_DEVICE float2 as_f2(unsigned long long a) { return *reinterpret_cast<float2*>(&a); }
+DFB_DEVICE float2 both(float a) { return make_float2(a, a); }
+DFB_DEVICE float2 mul2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(as_u64(a)), "l"(as_u64(b)));
+  return as_f2(r);
+}
+DFB_DEVICE float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(as_u64(a)), "l"(as_u64(b)), "l"(as_u64(c)));
+  return as_f2(r);
+}
+DFB_DEVICE float min_nan(float a, float b) {      // the smaller one, or NaN if either is
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+DFB_DEVICE float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // Byte of (row, block of 32) inside the tiled scales: tiles of 128 rows x 4 blocks, 512 bytes each, `tile_cols` tiles per
 // row of tiles (an even number, so that two tiles = 256 elements of K are one aligned kilobyte).
 DFB_DEVICE long long mx_scale_at(long long row, int block, int tile_cols) {
@@ -27,8 +53,30 @@ DFB_DEVICE float mx_scale_inv(uint32_t byte) { return __uint_as_float((254u - mi
 DFB_DEVICE float mx_scale_value(uint32_t byte) {
   return __uint_as_float(byte == 255u ? 0x7fc00000u : byte == 0u ? 0x00400000u : byte << 23);
 }
-// |x| for a block maximum in which NaN counts as infinity (fmaxf would drop it)
-DFB_DEVICE float mx_abs(float x) { return x == x ? fabsf(x) : INFINITY; }
+// largest magnitude of eight values; NaN if one is (its exponent is that of an infinity)
+DFB_DEVICE float mx_amax8(const float* f) {
+  float a = fabsf(f[0]);
+#pragma unroll
+  for (int i = 1; i < 8; ++i) a = max_nan(a, fabsf(f[i]));
+  return a;
+}
+// over the four neighbouring lanes that hold a block
+DFB_DEVICE float mx_amax4lanes(float a) {
+  a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));
+  return max_nan(a, __shfl_xor_sync(0xffffffffu, a, 2));
+}
+// f *= 2^k in pairs, then the codes
+DFB_DEVICE uint32_t mx_pack8(const float* f);
+DFB_DEVICE uint32_t mx_scale_pack8(const float* f, float inv) {
+  float g[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = mul2(make_float2(f[2 * i], f[2 * i + 1]), both(inv));
+    g[2 * i] = v.x;
+    g[2 * i + 1] = v.y;
+  }
+  return mx_pack8(g);
+}
 
 // eight e2m1 codes, element 0 in the lowest nibble; round to nearest even, saturating
 DFB_DEVICE uint32_t mx_pack8(const float* f) {

@@ -41,6 +41,23 @@ DFB_DEVICE Raw8<float> load8(const float* p, int live) {
   }
   return r;
 }
+// Largest magnitudes as bits, which order like the numbers, with NaN above infinity.  bf16: two neighbours in one instruction.
+DFB_DEVICE uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+DFB_DEVICE uint32_t words(const Raw8<bf16>& r, int j) { return *reinterpret_cast<const uint32_t*>(&r.v.v[j]); }
+DFB_DEVICE float amax8(const Raw8<bf16>& r) {
+  uint32_t a = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) a = max_u16x2(a, words(r, j) & 0x7fff7fffu);
+  return __uint_as_float(max(a << 16, a & 0xffff0000u));
+}
+DFB_DEVICE float amax8(const Raw8<float>& r) {
+  const float f[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+  return mx_amax8(f);
+}
 DFB_DEVICE void widen(const Raw8<bf16>& r, float* f) { unpack8(r.v, f); }
 DFB_DEVICE void widen(const Raw8<float>& r, float* f) {
   f[0] = r.a.x; f[1] = r.a.y; f[2] = r.a.z; f[3] = r.a.w;
@@ -52,25 +69,18 @@ DFB_DEVICE void widen(const Raw8<float>& r, float* f) {
 constexpr int kUnroll = 4;
 template <typename T, bool FULL>
 DFB_DEVICE void quant_rows(const T* x, long long ldx, uint8_t* q, uint8_t* tiles, long long rows, int K) {
-  const int tile_cols = mx_tile_cols(K), k = blockIdx.y * 256 + (threadIdx.x & 31) * 8;
-  const long long row0 = blockIdx.x * (8LL * kUnroll) + (threadIdx.x >> 5) * kUnroll;
+  const int tile_cols = mx_tile_cols(K), k = blockIdx.x * 256 + (threadIdx.x & 31) * 8;
+  const long long row0 = blockIdx.y * (8LL * kUnroll) + (threadIdx.x >> 5) * kUnroll;
   Raw8<T> raw[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) raw[u] = load8<FULL>(x + (row0 + u) * ldx + k, row0 + u < rows ? K - k : 0);
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     const long long row = row0 + u;
-    float f[8], amax = 0.f;
+    float f[8];
     widen(raw[u], f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, mx_abs(f[i]));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const uint32_t sb = mx_scale_byte(amax);
-    const float inv = mx_scale_inv(sb);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] *= inv;
-    if (FULL || (row < rows && k < K)) *reinterpret_cast<uint32_t*>(q + row * (K >> 1) + (k >> 1)) = mx_pack8(f);
+    const uint32_t sb = mx_scale_byte(mx_amax4lanes(amax8(raw[u])));
+    if (FULL || (row < rows && k < K)) *reinterpret_cast<uint32_t*>(q + row * (K >> 1) + (k >> 1)) = mx_scale_pack8(f, mx_scale_inv(sb));
     const uint32_t word = mx_scale_word(sb);
     if ((threadIdx.x & 15) == 0) *reinterpret_cast<uint32_t*>(tiles + mx_scale_at(row, k >> 5, tile_cols)) = word;
   }
@@ -78,7 +88,7 @@ DFB_DEVICE void quant_rows(const T* x, long long ldx, uint8_t* q, uint8_t* tiles
 template <typename T>
 __global__ void __launch_bounds__(256) quant_mxfp4_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q,
                                                            uint8_t* __restrict__ tiles, long long rows, int K, bool vec) {
-  if (vec && (blockIdx.x + 1) * (8LL * kUnroll) <= rows && static_cast<int>(blockIdx.y + 1) * 256 <= K) quant_rows<T, true>(x, ldx, q, tiles, rows, K);
+  if (vec && (blockIdx.y + 1) * (8LL * kUnroll) <= rows && static_cast<int>(blockIdx.x + 1) * 256 <= K) quant_rows<T, true>(x, ldx, q, tiles, rows, K);
   else quant_rows<T, false>(x, ldx, q, tiles, rows, K);
 }
 
@@ -94,24 +104,34 @@ DFB_DEVICE void quant_cols(const T* x, long long ldx, long long rows, int K, uin
   Raw8<T> raw[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) raw[k] = load8<FULL>(x + (kb + k) * ldx + n, live);
-  float f[8][8];                               // [k][row]
+  float f[8][8], amax[8];                      // [k][row]
 #pragma unroll
   for (int k = 0; k < 8; ++k) widen(raw[k], f[k]);
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t a = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) a = max_u16x2(a, words(raw[k], j) & 0x7fff7fffu);
+      a = max_u16x2(a, __shfl_xor_sync(0xffffffffu, a, 8));
+      a = max_u16x2(a, __shfl_xor_sync(0xffffffffu, a, 16));
+      amax[2 * j] = __uint_as_float(a << 16);
+      amax[2 * j + 1] = __uint_as_float(a & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const float g[8] = {f[0][r], f[1][r], f[2][r], f[3][r], f[4][r], f[5][r], f[6][r], f[7][r]};
+      float a = mx_amax8(g);
+      a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 8));
+      amax[r] = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 16));
+    }
+  }
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
-    float amax = 0.f, g[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      g[k] = f[k][r];
-      amax = fmaxf(amax, mx_abs(g[k]));
-    }
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 8));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 16));
-    const uint32_t sb = mx_scale_byte(amax);
-    const float inv = mx_scale_inv(sb);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) g[k] *= inv;
-    codes[grp * 8 + r][warp * 4 + sub] = mx_pack8(g);
+    const float g[8] = {f[0][r], f[1][r], f[2][r], f[3][r], f[4][r], f[5][r], f[6][r], f[7][r]};
+    const uint32_t sb = mx_scale_byte(amax[r]);
+    codes[grp * 8 + r][warp * 4 + sub] = mx_scale_pack8(g, mx_scale_inv(sb));
     if (sub == 0) scales[grp * 8 + r][warp] = static_cast<uint8_t>(sb);
   }
 }
@@ -177,7 +197,17 @@ int quant_mxfp4(const void* x, long long ldx, int x_f32, int transposed, void* q
   const long long rows_pad = (rows + 127) / 128 * 128;
   const long long gx = rows_pad / (transposed ? 64 : 8 * kUnroll);
   if (gx > 0x7fffffffLL || segs > 65535) return -3;
-  const dim3 grid(static_cast<unsigned>(gx), segs);
+  // along the rows the segments of a row come first (y: groups of 32 rows); along the columns the row tiles
+  if (!transposed && gx > 65535) {           // more rows than a grid's second axis holds: in slices of whole tiles
+    const long long part = 65535 / 4 * 128;  // a multiple of 128 rows
+    for (long long r = 0; r < rows; r += part) {
+      const int rc = quant_mxfp4(static_cast<const char*>(x) + r * ldx * es, ldx, x_f32, 0, static_cast<char*>(q) + r * (K / 2),
+                                 static_cast<char*>(tiles) + (r >> 7) * mx_tile_cols(K) * 512LL, rows - r < part ? rows - r : part, K, s);
+      if (rc) return rc;
+    }
+    return 0;
+  }
+  const dim3 grid = transposed ? dim3(static_cast<unsigned>(gx), segs) : dim3(segs, static_cast<unsigned>(gx));
   auto go = [&](auto kernel, auto* p) { kernel<<<grid, 256, 0, s>>>(p, ldx, (uint8_t*)q, (uint8_t*)tiles, rows, K, vec); };
   if (x_f32) {
     if (transposed) go(quant_mxfp4_cols_kernel<float>, (const float*)x);

@@ -12,8 +12,8 @@
 namespace dfb {
 namespace {
 
-// max / sum over the T threads of a row; every thread gets the result.  `part` holds one value per warp of the row and is
-// written once per kernel, so a single barrier is enough.
+// max / sum over the T threads of a row; every thread gets the result.  `part` holds one value per warp of the row and is not
+// written again before every thread has read it, so a single barrier is enough.
 template <int T, bool MAX>
 DFB_DEVICE float row_reduce(float v, float* part) {
   v = MAX ? warp_max(v) : warp_sum(v);
@@ -32,44 +32,52 @@ DFB_DEVICE void zero_scale_tail(uint8_t* tiles, long long row, bool dead, int bl
   for (int b = (dead ? 0 : (blocks + 3) / 4 * 4) + tid; b < tile_cols * 4; b += threads) tiles[mx_scale_at(row, b, tile_cols)] = 0;
 }
 
+// h = bf16(x + residual): the exact sum rounded once (the sum in 32 bits, rounded again, is the same number)
 DFB_DEVICE void add_round(bf16x8& a, const bf16x8& b) {
-  float f[8], g[8];
-  unpack8(a, f);
-  unpack8(b, g);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] += g[i];
-  a = pack8(f);
+  for (int i = 0; i < 4; ++i)
+    asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(*reinterpret_cast<uint32_t*>(&a.v[i]))
+        : "r"(*reinterpret_cast<const uint32_t*>(&a.v[i])), "r"(*reinterpret_cast<const uint32_t*>(&b.v[i])));
+}
+DFB_DEVICE float2 wide2(__nv_bfloat162 v) {
+  const uint32_t u = *reinterpret_cast<const uint32_t*>(&v);
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+DFB_DEVICE float sum_squares(const bf16x8& h) {
+  float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = wide2(h.v[i]);
+    s = fma2(f, f, s);
+  }
+  return s.x + s.y;
 }
 DFB_DEVICE void scaled(const bf16x8& h, const bf16x8& w, float r, float* f) {
-  float g[8];
-  unpack8(h, f);
-  unpack8(w, g);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = f[i] * r * g[i];
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = mul2(mul2(wide2(h.v[i]), both(r)), wide2(w.v[i]));
+    f[2 * i] = v.x;
+    f[2 * i + 1] = v.y;
+  }
 }
 // eight columns of y into the output format; `on` = these columns exist.  mxfp4: four neighbouring lanes hold a block.
 template <bool MX>
-DFB_DEVICE void emit(float* f, float inv, bool on, uint8_t* q, uint8_t* tiles, long long row, int v, int cols, int tile_cols) {
+DFB_DEVICE void emit(const float* f, float inv, bool on, uint8_t* q, uint8_t* tiles, long long row, int v, int cols, int tile_cols) {
   if constexpr (MX) {
-    float amax = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, mx_abs(f[i]));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const uint32_t sb = mx_scale_byte(amax);
-    const float iv = mx_scale_inv(sb);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] *= iv;
+    const uint32_t sb = mx_scale_byte(mx_amax4lanes(mx_amax8(f)));
     const uint32_t word = mx_scale_word(sb);          // columns that do not exist count as zero blocks
     if (on) {
-      *reinterpret_cast<uint32_t*>(q + row * (cols >> 1) + v * 4) = mx_pack8(f);
+      *reinterpret_cast<uint32_t*>(q + row * (cols >> 1) + v * 4) = mx_scale_pack8(f, mx_scale_inv(sb));
       if ((v & 15) == 0) *reinterpret_cast<uint32_t*>(tiles + mx_scale_at(row, v >> 2, tile_cols)) = word;
     }
   } else if (on) {
-    uint2 p;
-    p.x = e4m3_pack2(f[0] * inv, f[1] * inv) | e4m3_pack2(f[2] * inv, f[3] * inv) << 16;
-    p.y = e4m3_pack2(f[4] * inv, f[5] * inv) | e4m3_pack2(f[6] * inv, f[7] * inv) << 16;
-    *reinterpret_cast<uint2*>(q + row * cols + v * 8) = p;
+    uint32_t c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 y = mul2(make_float2(f[2 * i], f[2 * i + 1]), both(inv));
+      c[i] = e4m3_pack2(y.x, y.y);
+    }
+    *reinterpret_cast<uint2*>(q + row * cols + v * 8) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
   }
 }
 
@@ -88,79 +96,77 @@ struct NormArgs {
   float eps;
 };
 
-// T threads hold a row in registers, VPT vectors of eight columns each; a block takes max(1, 128 / T) rows.
+// T threads hold a row in registers, VPT vectors of eight columns each, and walk over rows with the next row's loads in flight
+// (one row per block left a gap between a row's loads and the last block's stores: 88 us at 16384 x 4096, now 80); the gain stays
+// in registers.  A block takes max(1, 128 / T) rows at a time.
 template <bool MX, bool RES, int T, int VPT>
-__global__ void __launch_bounds__(T < 128 ? 128 : T) rmsnorm_quant_kernel(const __grid_constant__ NormArgs a) {
-  __shared__ float part[2][T / 32];
+__global__ void __launch_bounds__(T < 128 ? 128 : T, T <= 256 ? 1024 / (T < 128 ? 128 : T) : 1)
+rmsnorm_quant_kernel(const __grid_constant__ NormArgs a) {
+  __shared__ float part[2][2][T / 32];             // [sum | max][parity of the row]: the next row's writes never meet this row's reads
+  static_assert(T == 32 || T >= 128, "a row is one warp (no barrier) or a whole block");
   constexpr int kRows = T < 128 ? 128 / T : 1;
   const int tid = threadIdx.x % T, nvec = a.cols >> 3, tile_cols = mx_tile_cols(a.cols);
-  const long long row = blockIdx.x * static_cast<long long>(kRows) + threadIdx.x / T;
-  if (MX) zero_scale_tail(a.tiles, row, row >= a.rows, a.cols / kMxBlock, tile_cols, tid, T);
-  if (row >= a.rows) return;                       // whole warps, and whole blocks where a row needs a barrier
-  bf16x8 h[VPT], w[VPT];
-#pragma unroll
-  for (int j = 0; j < VPT; ++j) {
-    const int v = j * T + tid;
-    h[j] = bf16x8{};
-    if (v < nvec) h[j] = ld8(a.x + row * a.ldx + v * 8);
-  }
-  if (RES) {
-    bf16x8 r[VPT];
+  const long long step = static_cast<long long>(gridDim.x) * kRows, rows_pad = MX ? (a.rows + 127) / 128 * 128 : a.rows;
+  long long row = blockIdx.x * static_cast<long long>(kRows) + threadIdx.x / T;
+  bf16x8 w[VPT], x[VPT], res[VPT];
+  auto fetch = [&](long long at) {
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       const int v = j * T + tid;
-      r[j] = bf16x8{};
-      if (v < nvec) r[j] = ld8(a.res + row * a.ldr + v * 8);
+      x[j] = bf16x8{};
+      if (v < nvec) x[j] = ld8(a.x + at * a.ldx + v * 8);
+      if (RES) {
+        res[j] = bf16x8{};
+        if (v < nvec) res[j] = ld8(a.res + at * a.ldr + v * 8);
+      }
     }
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-      const int v = j * T + tid;
-      add_round(h[j], r[j]);
-      if (v < nvec) st8(a.h + row * a.ldh + v * 8, h[j]);
-    }
-  }
+  };
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
     const int v = j * T + tid;
     w[j] = bf16x8{};
     if (v < nvec) w[j] = ld8(a.w + v * 8);
   }
-  float r;
-  if (a.rstd_in) {
-    r = a.rstd_in[row];
-  } else {
-    float ss = 0.f;
+  if (row < a.rows) fetch(row);
+  for (int it = 0; row < rows_pad; row += step, it ^= 1) {
+    if (MX) zero_scale_tail(a.tiles, row, row >= a.rows, a.cols / kMxBlock, tile_cols, tid, T);
+    if (row >= a.rows) continue;                   // whole warps, and whole blocks where a row needs a barrier
+    bf16x8 h[VPT];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-      float f[8];
-      unpack8(h[j], f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss += f[i] * f[i];
+      h[j] = x[j];
+      if (RES) {
+        add_round(h[j], res[j]);
+        if (j * T + tid < nvec) st8(a.h + row * a.ldh + (j * T + tid) * 8, h[j]);
+      }
     }
-    r = rsqrtf(row_reduce<T, false>(ss, part[0]) / a.cols + a.eps);
-    if (tid == 0) a.rstd_out[row] = r;
-  }
-  float inv = 1.f;
-  if (!MX) {
-    float amax = 0.f;
+    if (row + step < a.rows) fetch(row + step);
+    float r;
+    if (a.rstd_in) {
+      r = a.rstd_in[row];
+    } else {
+      float ss = 0.f;
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-      float f[8];
-      scaled(h[j], w[j], r, f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(f[i]));
+      for (int j = 0; j < VPT; ++j) ss += sum_squares(h[j]);
+      r = rsqrtf(row_reduce<T, false>(ss, part[0][it]) / a.cols + a.eps);
+      if (tid == 0) a.rstd_out[row] = r;
     }
-    amax = row_reduce<T, true>(amax, part[1]);
-    const float s = amax > 0.f ? fmaxf(__fmul_rn(amax, 1.f / kE4M3Top), kMinScale) : 1.f;
-    inv = __frcp_rn(s);
-    if (tid == 0) a.scale[row] = s;
-  }
+    float inv = 1.f, y[VPT][8];
 #pragma unroll
-  for (int j = 0; j < VPT; ++j) {
-    const int v = j * T + tid;
-    float f[8];
-    scaled(h[j], w[j], r, f);
-    emit<MX>(f, inv, v < nvec, a.q, a.tiles, row, v, a.cols, tile_cols);
+    for (int j = 0; j < VPT; ++j) scaled(h[j], w[j], r, y[j]);
+    if (!MX) {
+      float amax = 0.f;
+#pragma unroll
+      for (int j = 0; j < VPT; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(y[j][i]));
+      amax = row_reduce<T, true>(amax, part[1][it]);
+      const float s = amax > 0.f ? fmaxf(__fmul_rn(amax, 1.f / kE4M3Top), kMinScale) : 1.f;
+      inv = __frcp_rn(s);
+      if (tid == 0) a.scale[row] = s;
+    }
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) emit<MX>(y[j], inv, j * T + tid < nvec, a.q, a.tiles, row, j * T + tid, a.cols, tile_cols);
   }
 }
 
@@ -181,10 +187,7 @@ __global__ void __launch_bounds__(512) rmsnorm_quant_wide_kernel(const __grid_co
         add_round(h, ld8(a.res + row * a.ldr + v * 8));
         st8(a.h + row * a.ldh + v * 8, h);
       }
-      float f[8];
-      unpack8(h, f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss += f[i] * f[i];
+      ss += sum_squares(h);
     }
   }
   float r;
@@ -217,36 +220,38 @@ __global__ void __launch_bounds__(512) rmsnorm_quant_wide_kernel(const __grid_co
 }
 
 template <bool MX, bool RES>
-int launch(const NormArgs& a, cudaStream_t s) {
+int launch(const NormArgs& a, int num_sms, cudaStream_t s) {
   if (!a.rows) return 0;
   const long long rows = MX ? (a.rows + 127) / 128 * 128 : a.rows;      // with the padding of the scale tiles
   if (rows > 0x7fffffffLL) return -3;
   const int nvec = a.cols >> 3;
+  // as many blocks as stay resident: 1024 threads per SM
   auto go = [&](auto kernel, int threads, int rows_per_block) {
-    kernel<<<static_cast<unsigned>((rows + rows_per_block - 1) / rows_per_block), threads, 0, s>>>(a);
+    const long long need = (rows + rows_per_block - 1) / rows_per_block, fit = static_cast<long long>(num_sms) * (1024 / threads);
+    kernel<<<static_cast<unsigned>(need < fit ? need : fit), threads, 0, s>>>(a);
   };
   if (nvec <= 32) go(rmsnorm_quant_kernel<MX, RES, 32, 1>, 128, 4);
   else if (nvec <= 64) go(rmsnorm_quant_kernel<MX, RES, 32, 2>, 128, 4);
   else if (nvec <= 128) go(rmsnorm_quant_kernel<MX, RES, 32, 4>, 128, 4);
   else if (nvec <= 256) go(rmsnorm_quant_kernel<MX, RES, 128, 2>, 128, 1);
-  else if (nvec <= 512) go(rmsnorm_quant_kernel<MX, RES, 128, 4>, 128, 1);
-  else if (nvec <= 1024) go(rmsnorm_quant_kernel<MX, RES, 256, 4>, 256, 1);
-  else if (nvec <= 2048) go(rmsnorm_quant_kernel<MX, RES, 512, 4>, 512, 1);
-  else go(rmsnorm_quant_wide_kernel<MX, RES>, 512, 1);
+  else if (nvec <= 512) go(rmsnorm_quant_kernel<MX, RES, 256, 2>, 256, 1);
+  else if (nvec <= 1024) go(rmsnorm_quant_kernel<MX, RES, 512, 2>, 512, 1);
+  else if (nvec <= 2048) go(rmsnorm_quant_kernel<MX, RES, 1024, 2>, 1024, 1);
+  else rmsnorm_quant_wide_kernel<MX, RES><<<static_cast<unsigned>(rows), 512, 0, s>>>(a);
   return cudaGetLastError() == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace
 
 int rmsnorm_fp8(const void* x, long long ldx, const void* res, long long ldr, const void* w, const float* rstd_in, float eps, void* h,
-                long long ldh, void* q, float* scale, float* rstd, long long rows, int cols, cudaStream_t s) {
+                long long ldh, void* q, float* scale, float* rstd, long long rows, int cols, int num_sms, cudaStream_t s) {
   const NormArgs a{(const bf16*)x, (const bf16*)res, (const bf16*)w, rstd_in, (bf16*)h, (uint8_t*)q, scale, nullptr, rstd, ldx, ldr, ldh, rows, cols, eps};
-  return res ? launch<false, true>(a, s) : launch<false, false>(a, s);
+  return res ? launch<false, true>(a, num_sms, s) : launch<false, false>(a, num_sms, s);
 }
 int rmsnorm_mxfp4(const void* x, long long ldx, const void* res, long long ldr, const void* w, const float* rstd_in, float eps, void* h,
-                  long long ldh, void* q, void* tiles, float* rstd, long long rows, int cols, cudaStream_t s) {
+                  long long ldh, void* q, void* tiles, float* rstd, long long rows, int cols, int num_sms, cudaStream_t s) {
   const NormArgs a{(const bf16*)x, (const bf16*)res, (const bf16*)w, rstd_in, (bf16*)h, (uint8_t*)q, nullptr, (uint8_t*)tiles, rstd, ldx, ldr, ldh, rows, cols, eps};
-  return res ? launch<true, true>(a, s) : launch<true, false>(a, s);
+  return res ? launch<true, true>(a, num_sms, s) : launch<true, false>(a, num_sms, s);
 }
 
 }  // namespace dfb

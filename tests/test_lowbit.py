@@ -159,7 +159,7 @@ def product_bound(A, B, K, out):
 @pytest.mark.parametrize("dev", LANES)
 @pytest.mark.parametrize("out", [BF, F32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("M,N,K", [(1, 1, 32), (1, 8, 64), (3, 7, 96), (128, 128, 256), (129, 257, 288), (17, 520, 1056), (300, 40, 544),
-                                   (257, 264, 2048), (130, 72, 32), (640, 513, 160), (2309, 4104, 96)])
+                                   (257, 264, 2048), (130, 72, 32), (640, 513, 160), (65, 300, 4128), (2309, 4104, 544), (2100, 4099, 64)])
 def test_product(dev, out, M, N, K):
     k = lane(dev)
     x = rnd(dev, M, K, seed=M, dtype=F32) * torch.exp(rnd(dev, M, 1, seed=2, dtype=F32))
@@ -502,21 +502,18 @@ def test_adamw_nan_and_zero_gradients(dev):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("form", FORMS)
-def test_adamw_kernel_and_plain_lane_agree_in_8_bit_state(form):
-    """The lanes differ by a fused product-sum and by the kernel's root (within 2^-23): y is within 8 u of the other lane's, so a
-    code differs where y lies that near to a border: a share of at most 2 * 8 u * 16 = 2^-16 of the elements (16: the grid steps
-    that a y holds), 1.1 of 74225 expected per moment."""
+def test_adamw_kernel_and_plain_lane_agree_to_the_bit_in_8_bit_state(form):
+    """The arithmetic in front of the rounding is the same sequence of rounded fp32 operations in both lanes."""
     sizes = [70000, 129, 4096]
     st = opt_state("cuda", sizes, form, BF, 8, seed=11)
     ref = clone(st)
     for s, K in ((st, lane("cuda")), (ref, resolve_kernels(kernel_set="eager").lowbit)):
-        K.adamw_multi_step(s["ws"], s["gs"], s["ms"], s["vs"], 1e-3, wds=0.1, step=1,
-                           **{n: s[n] for n in ("masters", "los", "m_scales", "v_scales") if n in s})
-    for n in ("ms", "vs"):
-        assert sum(int((a.view(U8) != b.view(U8)).sum()) for a, b in zip(st[n], ref[n])) <= 12
-    for n in ("m_scales", "v_scales"):
+        for step in (1, 2, 3):
+            K.adamw_multi_step(s["ws"], s["gs"], s["ms"], s["vs"], 1e-3, wds=0.1, step=step,
+                               **{n: s[n] for n in ("masters", "los", "m_scales", "v_scales") if n in s})
+    for n in ("ms", "vs", "m_scales", "v_scales"):
         for a, b in zip(st[n], ref[n]):
-            assert ((a - b).abs() <= 8 * U * b).all()
+            assert torch.equal(a.view(U8), b.view(U8)), n
 
 
 # ------------------------------------------------------------------ refusals: the plain lane, and the extension on host tensors
