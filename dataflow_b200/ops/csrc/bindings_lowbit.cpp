@@ -2,6 +2,7 @@
 // device check, so that a refusal can be tested on host tensors; a call that passes launches on the device of its operands and
 // on that device's current stream.  Refused arguments raise ValueError.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -46,6 +47,9 @@ void on_device(const char* op, std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts) REFUSE_UNLESS(t->device() == first->device(), op, ": operands are on different devices");
   REFUSE_UNLESS(first->is_cuda(), op, ": operands must be CUDA tensors");
 }
+Tensor empty_like_device(at::IntArrayRef sizes, at::ScalarType dt, const Tensor& t) {      // at::empty without the dispatcher
+  return at::detail::empty_cuda(sizes, dt, t.device(), c10::nullopt);
+}
 int sms(const Tensor& t) { return at::cuda::getDeviceProperties(t.device().index())->multiProcessorCount; }
 cudaStream_t stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 void launched(int rc, const char* op) { TORCH_CHECK(rc == 0, op, " failed to launch (code ", rc, ")"); }
@@ -84,8 +88,7 @@ std::tuple<Tensor, Tensor> quant_mxfp4(const Tensor& x, bool transpose) {
   REFUSE_UNLESS(ld >= x.size(1), "quant_mxfp4: rows of x must not overlap");
   on_device("quant_mxfp4", {&x});
   c10::cuda::CUDAGuard guard(x.device());
-  auto u8 = x.options().dtype(at::kByte);
-  Tensor q = at::empty({rows, K / 2}, u8), s = at::empty({(rows + 127) / 128, tile_cols(K), 512}, u8);
+  Tensor q = empty_like_device({rows, K / 2}, at::kByte, x), s = empty_like_device({(rows + 127) / 128, tile_cols(K), 512}, at::kByte, x);
   launched(dfb::quant_mxfp4(x.const_data_ptr(), ld, f32, transpose, q.data_ptr(), s.data_ptr(), rows, (int)K, stream_of(x)), "quant_mxfp4");
   return {q, s};
 }
@@ -95,7 +98,7 @@ Tensor dequant_mxfp4(const Tensor& q, const Tensor& scale, at::ScalarType dt) {
   REFUSE_UNLESS(dt == at::kBFloat16 || dt == at::kFloat, "dequant_mxfp4: values are bf16 or fp32");
   on_device("dequant_mxfp4", {&q, &scale});
   c10::cuda::CUDAGuard guard(q.device());
-  Tensor y = at::empty({q.size(0), q.size(1) * 2}, q.options().dtype(dt));
+  Tensor y = empty_like_device({q.size(0), q.size(1) * 2}, dt, q);
   launched(dfb::dequant_mxfp4(q.const_data_ptr(), scale.const_data_ptr(), y.data_ptr(), dt == at::kFloat, q.size(0), (int)q.size(1) * 2, stream_of(q)),
            "dequant_mxfp4");
   return y;
@@ -130,7 +133,7 @@ Tensor linear_mxfp4(const Tensor& xq, const Tensor& xs, const Tensor& wq, const 
   }
   on_device("linear_mxfp4", {&xq, &xs, &wq, &ws, out.has_value() ? &*out : &xq, add.has_value() ? &*add : &xq, bias.has_value() ? &*bias : &xq});
   c10::cuda::CUDAGuard guard(xq.device());
-  Tensor d = out.has_value() ? *out : at::empty({M, N}, xq.options().dtype(dt));
+  Tensor d = out.has_value() ? *out : empty_like_device({M, N}, dt, xq);
   launched(dfb::gemm_mxfp4(xq.const_data_ptr(), xs.const_data_ptr(), wq.const_data_ptr(), ws.const_data_ptr(), d.data_ptr(), ld(d), dt == at::kFloat,
                            add.has_value() ? add->const_data_ptr() : nullptr, add.has_value() ? ld(*add) : 0,
                            bias.has_value() ? bias->const_data_ptr() : nullptr, M, N, (int)xq.size(1) * 2, sms(xq), stream_of(xq)),
@@ -172,20 +175,19 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rmsnorm_narrow(bool mx, const Tensor&
   }
   on_device(op, {&x, &w, residual.has_value() ? &*residual : &x, rstd_in.has_value() ? &*rstd_in : &x, h_out.has_value() ? &*h_out : &x});
   c10::cuda::CUDAGuard guard(x.device());
-  Tensor h = !residual.has_value() ? x : h_out.has_value() ? *h_out : at::empty(x.sizes(), x.options());
-  Tensor rstd = rstd_in.has_value() ? rstd_in->view({rows}) : at::empty({rows}, x.options().dtype(at::kFloat));
+  Tensor h = !residual.has_value() ? x : h_out.has_value() ? *h_out : empty_like_device(x.sizes(), at::kBFloat16, x);
+  Tensor rstd = rstd_in.has_value() ? rstd_in->view({rows}) : empty_like_device({rows}, at::kFloat, x);
   float* rstd_out = rstd_in.has_value() ? nullptr : rstd.data_ptr<float>();
   const float* given = rstd_in.has_value() ? rstd_in->const_data_ptr<float>() : nullptr;
   const void* rp = residual.has_value() ? residual->const_data_ptr() : nullptr;
   void* hp = residual.has_value() ? h.data_ptr() : nullptr;
   if (mx) {
-    auto u8 = x.options().dtype(at::kByte);
-    Tensor q = at::empty({rows, cols / 2}, u8), s = at::empty({(rows + 127) / 128, tile_cols(cols), 512}, u8);
+    Tensor q = empty_like_device({rows, cols / 2}, at::kByte, x), s = empty_like_device({(rows + 127) / 128, tile_cols(cols), 512}, at::kByte, x);
     launched(dfb::rmsnorm_mxfp4(x.const_data_ptr(), ldx, rp, ldr, w.const_data_ptr(), given, (float)eps, hp, ldh, q.data_ptr(), s.data_ptr(), rstd_out,
                                 rows, (int)cols, sms(x), stream_of(x)), op);
     return {q, s, h, rstd};
   }
-  Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn)), s = at::empty({rows}, x.options().dtype(at::kFloat));
+  Tensor q = empty_like_device(x.sizes(), at::kFloat8_e4m3fn, x), s = empty_like_device({rows}, at::kFloat, x);
   launched(dfb::rmsnorm_fp8(x.const_data_ptr(), ldx, rp, ldr, w.const_data_ptr(), given, (float)eps, hp, ldh, q.data_ptr(), s.data_ptr<float>(), rstd_out,
                             rows, (int)cols, sms(x), stream_of(x)), op);
   return {q, s, h, rstd};
@@ -268,7 +270,7 @@ void adamw_multi(const std::vector<Tensor>& ws, const std::vector<Tensor>& gs, c
   h.gscale = (float)gscale;
   h.seed = static_cast<uint32_t>(seed);
   const int weights = masters.has_value() ? dfb::kAdamMaster : los.has_value() ? dfb::kAdamSplit : wt == at::kFloat ? dfb::kAdamF32 : dfb::kAdamBf16;
-  launched(dfb::adamw_multi(table.data(), (int)table.size(), weights, gt == at::kFloat, bits8, h, stream_of(ws[0])), op);
+  launched(dfb::adamw_multi(table.data(), (int)table.size(), weights, gt == at::kFloat, bits8, h, sms(ws[0]), stream_of(ws[0])), op);
 }
 
 at::ScalarType dtype_of(const py::object& o) { return torch::python::detail::py_object_to_dtype(o); }

@@ -24,7 +24,7 @@ struct AdamHyper {
   uint32_t seed;
   float one = 1.f;
 };
-int adamw_multi(const AdamTensor* t, int count, int weights, bool g_f32, bool bits8, const AdamHyper& h, cudaStream_t s);
+int adamw_multi(const AdamTensor* t, int count, int weights, bool g_f32, bool bits8, const AdamHyper& h, int num_sms, cudaStream_t s);
 
 // h = bf16(x + residual) (h == null: x is taken as it is), y = h * rstd * w.  rstd_in: statistics to apply (null: computed).
 int rmsnorm_fp8(const void* x, long long ldx, const void* res, long long ldr, const void* w, const float* rstd_in, float eps, void* h,

@@ -71,18 +71,21 @@ template <typename T, bool FULL>
 DFB_DEVICE void quant_rows(const T* x, long long ldx, uint8_t* q, uint8_t* tiles, long long rows, int K) {
   const int tile_cols = mx_tile_cols(K), k = blockIdx.x * 256 + (threadIdx.x & 31) * 8;
   const long long row0 = blockIdx.y * (8LL * kUnroll) + (threadIdx.x >> 5) * kUnroll;
+  const int left = static_cast<int>(rows - row0 < kUnroll ? (rows > row0 ? rows - row0 : 0) : kUnroll);
+  const T* xp = x + row0 * ldx + k;
+  uint8_t* qp = q + row0 * (K >> 1) + (k >> 1);
+  uint8_t* tile = tiles + mx_scale_at(row0, k >> 5, tile_cols);      // kUnroll rows inside a group of 32: 16 bytes apart
   Raw8<T> raw[kUnroll];
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) raw[u] = load8<FULL>(x + (row0 + u) * ldx + k, row0 + u < rows ? K - k : 0);
+  for (int u = 0; u < kUnroll; ++u) raw[u] = load8<FULL>(xp + u * ldx, FULL || u < left ? K - k : 0);
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    const long long row = row0 + u;
     float f[8];
     widen(raw[u], f);
     const uint32_t sb = mx_scale_byte(mx_amax4lanes(amax8(raw[u])));
-    if (FULL || (row < rows && k < K)) *reinterpret_cast<uint32_t*>(q + row * (K >> 1) + (k >> 1)) = mx_scale_pack8(f, mx_scale_inv(sb));
+    if (FULL || (u < left && k < K)) *reinterpret_cast<uint32_t*>(qp + u * static_cast<long long>(K >> 1)) = mx_scale_pack8(f, mx_scale_inv(sb));
     const uint32_t word = mx_scale_word(sb);
-    if ((threadIdx.x & 15) == 0) *reinterpret_cast<uint32_t*>(tiles + mx_scale_at(row, k >> 5, tile_cols)) = word;
+    if ((threadIdx.x & 15) == 0) *reinterpret_cast<uint32_t*>(tile + u * 16) = word;
   }
 }
 template <typename T>
@@ -160,25 +163,28 @@ __global__ void __launch_bounds__(256) dequant_mxfp4_kernel(const uint8_t* __res
                                                              T* __restrict__ y, long long rows, int K) {
   const int tile_cols = mx_tile_cols(K), k = blockIdx.y * 256 + (threadIdx.x & 31) * 8;
   const long long row0 = blockIdx.x * (8LL * kUnroll) + (threadIdx.x >> 5) * kUnroll;
-  if (k >= K) return;
+  if (k >= K || row0 >= rows) return;
+  const int left = static_cast<int>(rows - row0 < kUnroll ? rows - row0 : kUnroll);
+  const uint8_t* qp = q + row0 * (K >> 1) + (k >> 1);
+  const uint8_t* tile = tiles + mx_scale_at(row0, k >> 5, tile_cols);
   uint32_t c[kUnroll], sb[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     c[u] = sb[u] = 0;
-    if (row0 + u < rows) {
-      c[u] = *reinterpret_cast<const uint32_t*>(q + (row0 + u) * (K >> 1) + (k >> 1));
-      sb[u] = tiles[mx_scale_at(row0 + u, k >> 5, tile_cols)];
+    if (u < left) {
+      c[u] = *reinterpret_cast<const uint32_t*>(qp + u * static_cast<long long>(K >> 1));
+      sb[u] = tile[u * 16];
     }
   }
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    if (row0 + u >= rows) break;
+    if (u >= left) break;
     const float s = mx_scale_value(sb[u]);
     float f[8];
     mx_unpack8(c[u], f);
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] *= s;
-    T* yp = y + (row0 + u) * K + k;
+    T* yp = y + row0 * K + k + u * static_cast<long long>(K);
     if constexpr (sizeof(T) == 4) {
       *reinterpret_cast<float4*>(yp) = make_float4(f[0], f[1], f[2], f[3]);
       *reinterpret_cast<float4*>(yp + 4) = make_float4(f[4], f[5], f[6], f[7]);

@@ -27,9 +27,9 @@ DFB_DEVICE float row_reduce(float v, float* part) {
   return v;
 }
 
-// scale bytes past the rows and past the blocks are zero (the last word of a row's own blocks is written whole by emit)
-DFB_DEVICE void zero_scale_tail(uint8_t* tiles, long long row, bool dead, int blocks, int tile_cols, int tid, int threads) {
-  for (int b = (dead ? 0 : (blocks + 3) / 4 * 4) + tid; b < tile_cols * 4; b += threads) tiles[mx_scale_at(row, b, tile_cols)] = 0;
+// scale words past the rows and past the blocks are zero; emit writes the `words` words that hold a row's own blocks
+DFB_DEVICE void zero_scale_tail(uint8_t* tile, int words, int tile_cols, int tid, int threads) {
+  for (int t = words + tid; t < tile_cols; t += threads) *reinterpret_cast<uint32_t*>(tile + t * 512) = 0;
 }
 
 // h = bf16(x + residual): the exact sum rounded once (the sum in 32 bits, rounded again, is the same number)
@@ -60,15 +60,16 @@ DFB_DEVICE void scaled(const bf16x8& h, const bf16x8& w, float r, float* f) {
     f[2 * i + 1] = v.y;
   }
 }
-// eight columns of y into the output format; `on` = these columns exist.  mxfp4: four neighbouring lanes hold a block.
+// Eight columns of y into the output format; `on` = these columns exist, v = their index in eights, q / tile = where the row's
+// codes and its first scale word lie.  mxfp4: four neighbouring lanes hold a block, sixteen a word of scales; 512 bytes to the next.
 template <bool MX>
-DFB_DEVICE void emit(const float* f, float inv, bool on, uint8_t* q, uint8_t* tiles, long long row, int v, int cols, int tile_cols) {
+DFB_DEVICE void emit(const float* f, float inv, bool on, uint8_t* q, uint8_t* tile, int v) {
   if constexpr (MX) {
     const uint32_t sb = mx_scale_byte(mx_amax4lanes(mx_amax8(f)));
     const uint32_t word = mx_scale_word(sb);          // columns that do not exist count as zero blocks
     if (on) {
-      *reinterpret_cast<uint32_t*>(q + row * (cols >> 1) + v * 4) = mx_scale_pack8(f, mx_scale_inv(sb));
-      if ((v & 15) == 0) *reinterpret_cast<uint32_t*>(tiles + mx_scale_at(row, v >> 2, tile_cols)) = word;
+      *reinterpret_cast<uint32_t*>(q + v * 4) = mx_scale_pack8(f, mx_scale_inv(sb));
+      if ((v & 15) == 0) *reinterpret_cast<uint32_t*>(tile + (v >> 4) * 512) = word;
     }
   } else if (on) {
     uint32_t c[4];
@@ -77,7 +78,7 @@ DFB_DEVICE void emit(const float* f, float inv, bool on, uint8_t* q, uint8_t* ti
       const float2 y = mul2(make_float2(f[2 * i], f[2 * i + 1]), both(inv));
       c[i] = e4m3_pack2(y.x, y.y);
     }
-    *reinterpret_cast<uint2*>(q + row * cols + v * 8) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+    *reinterpret_cast<uint2*>(q + v * 8) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
   }
 }
 
@@ -93,7 +94,7 @@ struct NormArgs {
   float* rstd_out;
   long long ldx, ldr, ldh, rows;
   int cols;
-  float eps;
+  float eps, inv_cols;
 };
 
 // T threads hold a row in registers, VPT vectors of eight columns each, and walk over rows with the next row's loads in flight
@@ -109,27 +110,34 @@ rmsnorm_quant_kernel(const __grid_constant__ NormArgs a) {
   const long long step = static_cast<long long>(gridDim.x) * kRows, rows_pad = MX ? (a.rows + 127) / 128 * 128 : a.rows;
   long long row = blockIdx.x * static_cast<long long>(kRows) + threadIdx.x / T;
   bf16x8 w[VPT], x[VPT], res[VPT];
-  auto fetch = [&](long long at) {
+  // where this thread's part of the row being fetched lies; advanced row by row
+  const bf16 *xp = a.x + row * a.ldx + tid * 8, *rp = a.res + (RES ? row * a.ldr + tid * 8 : 0);
+  auto fetch = [&]() {
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-      const int v = j * T + tid;
+      const bool on = j * T + tid < nvec;
       x[j] = bf16x8{};
-      if (v < nvec) x[j] = ld8(a.x + at * a.ldx + v * 8);
+      if (on) x[j] = ld8(xp + j * (T * 8));
       if (RES) {
         res[j] = bf16x8{};
-        if (v < nvec) res[j] = ld8(a.res + at * a.ldr + v * 8);
+        if (on) res[j] = ld8(rp + j * (T * 8));
       }
     }
+    xp += step * a.ldx;
+    if (RES) rp += step * a.ldr;
   };
+  const int words = (a.cols + 127) >> 7;
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
     const int v = j * T + tid;
     w[j] = bf16x8{};
     if (v < nvec) w[j] = ld8(a.w + v * 8);
   }
-  if (row < a.rows) fetch(row);
+  if (row < a.rows) fetch();
   for (int it = 0; row < rows_pad; row += step, it ^= 1) {
-    if (MX) zero_scale_tail(a.tiles, row, row >= a.rows, a.cols / kMxBlock, tile_cols, tid, T);
+    uint8_t* tile = MX ? a.tiles + mx_scale_at(row, 0, tile_cols) : nullptr;
+    uint8_t* q = a.q + row * (MX ? a.cols >> 1 : a.cols);
+    if (MX && (words < tile_cols || row >= a.rows)) zero_scale_tail(tile, row < a.rows ? words : 0, tile_cols, tid, T);
     if (row >= a.rows) continue;                   // whole warps, and whole blocks where a row needs a barrier
     bf16x8 h[VPT];
 #pragma unroll
@@ -140,7 +148,7 @@ rmsnorm_quant_kernel(const __grid_constant__ NormArgs a) {
         if (j * T + tid < nvec) st8(a.h + row * a.ldh + (j * T + tid) * 8, h[j]);
       }
     }
-    if (row + step < a.rows) fetch(row + step);
+    if (row + step < a.rows) fetch();
     float r;
     if (a.rstd_in) {
       r = a.rstd_in[row];
@@ -148,7 +156,7 @@ rmsnorm_quant_kernel(const __grid_constant__ NormArgs a) {
       float ss = 0.f;
 #pragma unroll
       for (int j = 0; j < VPT; ++j) ss += sum_squares(h[j]);
-      r = rsqrtf(row_reduce<T, false>(ss, part[0][it]) / a.cols + a.eps);
+      r = rsqrtf(row_reduce<T, false>(ss, part[0][it]) * a.inv_cols + a.eps);
       if (tid == 0) a.rstd_out[row] = r;
     }
     float inv = 1.f, y[VPT][8];
@@ -166,7 +174,7 @@ rmsnorm_quant_kernel(const __grid_constant__ NormArgs a) {
       if (tid == 0) a.scale[row] = s;
     }
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) emit<MX>(y[j], inv, j * T + tid < nvec, a.q, a.tiles, row, j * T + tid, a.cols, tile_cols);
+    for (int j = 0; j < VPT; ++j) emit<MX>(y[j], inv, j * T + tid < nvec, q, tile, j * T + tid);
   }
 }
 
@@ -176,7 +184,9 @@ __global__ void __launch_bounds__(512) rmsnorm_quant_wide_kernel(const __grid_co
   __shared__ float part[2][16];
   const long long row = blockIdx.x;
   const int nvec = a.cols >> 3, tile_cols = mx_tile_cols(a.cols);
-  if (MX) zero_scale_tail(a.tiles, row, row >= a.rows, a.cols / kMxBlock, tile_cols, threadIdx.x, 512);
+  uint8_t* tile = MX ? a.tiles + mx_scale_at(row, 0, tile_cols) : nullptr;
+  uint8_t* q = a.q + row * (MX ? a.cols >> 1 : a.cols);
+  if (MX) zero_scale_tail(tile, row < a.rows ? (a.cols + 127) >> 7 : 0, tile_cols, threadIdx.x, 512);
   if (row >= a.rows) return;
   const bf16* hr = RES ? a.h + row * a.ldh : a.x + row * a.ldx;
   float ss = 0.f;
@@ -194,7 +204,7 @@ __global__ void __launch_bounds__(512) rmsnorm_quant_wide_kernel(const __grid_co
   if (a.rstd_in) {
     r = a.rstd_in[row];
   } else {
-    r = rsqrtf(row_reduce<512, false>(ss, part[0]) / a.cols + a.eps);
+    r = rsqrtf(row_reduce<512, false>(ss, part[0]) * a.inv_cols + a.eps);
     if (threadIdx.x == 0) a.rstd_out[row] = r;
   }
   float inv = 1.f;
@@ -215,7 +225,7 @@ __global__ void __launch_bounds__(512) rmsnorm_quant_wide_kernel(const __grid_co
     const int v = v0 + threadIdx.x;
     float f[8] = {};
     if (v < nvec) scaled(ld8(hr + v * 8), ld8(a.w + v * 8), r, f);
-    emit<MX>(f, inv, v < nvec, a.q, a.tiles, row, v, a.cols, tile_cols);
+    emit<MX>(f, inv, v < nvec, q, tile, v);
   }
 }
 
@@ -245,12 +255,12 @@ int launch(const NormArgs& a, int num_sms, cudaStream_t s) {
 
 int rmsnorm_fp8(const void* x, long long ldx, const void* res, long long ldr, const void* w, const float* rstd_in, float eps, void* h,
                 long long ldh, void* q, float* scale, float* rstd, long long rows, int cols, int num_sms, cudaStream_t s) {
-  const NormArgs a{(const bf16*)x, (const bf16*)res, (const bf16*)w, rstd_in, (bf16*)h, (uint8_t*)q, scale, nullptr, rstd, ldx, ldr, ldh, rows, cols, eps};
+  const NormArgs a{(const bf16*)x, (const bf16*)res, (const bf16*)w, rstd_in, (bf16*)h, (uint8_t*)q, scale, nullptr, rstd, ldx, ldr, ldh, rows, cols, eps, 1.f / cols};
   return res ? launch<false, true>(a, num_sms, s) : launch<false, false>(a, num_sms, s);
 }
 int rmsnorm_mxfp4(const void* x, long long ldx, const void* res, long long ldr, const void* w, const float* rstd_in, float eps, void* h,
                   long long ldh, void* q, void* tiles, float* rstd, long long rows, int cols, int num_sms, cudaStream_t s) {
-  const NormArgs a{(const bf16*)x, (const bf16*)res, (const bf16*)w, rstd_in, (bf16*)h, (uint8_t*)q, nullptr, (uint8_t*)tiles, rstd, ldx, ldr, ldh, rows, cols, eps};
+  const NormArgs a{(const bf16*)x, (const bf16*)res, (const bf16*)w, rstd_in, (bf16*)h, (uint8_t*)q, nullptr, (uint8_t*)tiles, rstd, ldx, ldr, ldh, rows, cols, eps, 1.f / cols};
   return res ? launch<true, true>(a, num_sms, s) : launch<true, false>(a, num_sms, s);
 }
 
