@@ -317,6 +317,11 @@ def test_norm_layouts_and_edges(dev):
     assert s[1] == 1 and (q[1].float() == 0).all() and torch.isnan(q[2].float()).all() and q[3].float().isfinite().all()
     v = unpack(k, *k.rmsnorm_mxfp4(x, w)[:2])
     assert (v[1] == 0).all() and torch.isnan(v[2]).all() and v[0].isfinite().all() and v[3].isfinite().all()
+    # sums of subnormal numbers are sums, and zeros keep their sign's rules
+    a = torch.tensor([1e-39, -1e-39, 3e-39, -0.0, 0.0, -0.0, 2e-38, 1.0] * 8).to(BF).to(dev).view(1, 64)
+    b = torch.tensor([1e-39, 5e-40, -3e-39, -0.0, -0.0, 0.0, -1.9e-38, 2.0 ** -9] * 8).to(BF).to(dev).view(1, 64)
+    h = k.rmsnorm_fp8(a, w, residual=b)[2]
+    assert torch.equal(h.view(torch.int16), (a.float().cpu() + b.float().cpu()).to(BF).to(dev).view(torch.int16))
     # a gain so small that 448 steps of it leave the normal numbers
     tiny = torch.full((64,), 2.0 ** -126, dtype=BF, device=dev)
     q, s, _, _ = k.rmsnorm_fp8(x[:1], tiny)

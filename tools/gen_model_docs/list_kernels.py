@@ -20,12 +20,14 @@ def main(argv=None) -> int:
     ap.add_argument("--kernel-set", default=None)
     a = ap.parse_args(argv)
     from dataflow_b200.ops import registered_ops, resolve_kernels
-    ks = resolve_kernels(kernel_set=a.kernel_set)
-    chosen = ks.describe()
-    rows = [{"op": op, "implementations": ", ".join(sorted(k.name for k in impls)), "resolved": chosen.get(op, "-"),
-             "native": "yes" if op in ks.native_ops() else ""} for op, impls in sorted(registered_ops().items())]
-    print(table(rows, [("op", "{}"), ("implementations", "{}"), ("resolved", "{}"), ("native", "{}")]))
-    print(f"{len(rows)} ops; {len(ks.native_ops())} resolve to native code here")
+    core = resolve_kernels(kernel_set=a.kernel_set)
+    for op_set, ks in (("core", core), ("lowbit", core.lowbit)):
+        chosen = ks.describe()
+        prefix = "" if op_set == "core" else f"{op_set}."
+        rows = [{"op": prefix + op, "implementations": ", ".join(sorted(k.name for k in impls)), "resolved": chosen.get(op, "-"),
+                 "native": "yes" if op in ks.native_ops() else ""} for op, impls in sorted(registered_ops(op_set).items())]
+        print(table(rows, [("op", "{}"), ("implementations", "{}"), ("resolved", "{}"), ("native", "{}")]))
+        print(f"{len(rows)} ops; {len(ks.native_ops())} resolve to native code here")
     return 0
 
 
