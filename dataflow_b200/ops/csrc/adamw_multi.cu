@@ -7,9 +7,10 @@
 // of e4m3's 6 to 12 % spacing, so rounding to nearest would never let it fall again.  The random bits are a hash of (element
 // index, seed).  A positive r keeps at least the smallest code.  The update itself uses the unrounded moments.
 //
-// The kernel moves 10 bytes per element with 8-bit moments (28 with fp32 moments and a master) and is bound by memory: a block
-// takes 4096 consecutive elements of one tensor, a thread eight or (8-bit moments) sixteen of them, so that eight lanes share a scale.  Tensors travel as a
-// table in the kernel's parameters (no copy, no device-side table that a captured graph would share); a block finds its tensor
+// The kernel moves 10 bytes per element with 8-bit moments (28 with fp32 moments and a master) and is bound by memory
+// (8 bits: 0.89 of the copy rate at 218M parameters, 379 us, with the arithmetic close behind: 45 instructions an element; 32 bits:
+// 1.0).  A block takes consecutive elements of one tensor, a thread eight or (8-bit moments) sixteen of them, so that eight lanes
+// share a scale.  Tensors travel as a table in the kernel's parameters (no copy, no device-side table that a captured graph would share); a block finds its tensor
 // by bisection.
 #include "lowbit.h"
 #include "lowbit_common.cuh"
@@ -17,15 +18,17 @@
 namespace dfb {
 namespace {
 
-// Elements of a block: 4096 where that makes blocks enough, else 1024 (8-bit moments) or 2048: one group per thread, the shortest
-// way through (a block's twelve small fields 4.3 us instead of 6.7).
-constexpr int kChunk = 4096;
-// Threads of a block, and blocks per SM.  The 8-bit form at 176M parameters: sixteen elements a thread, 64 threads, 10 blocks
-// (96 registers) 334 us; 128 threads at 4 / 5 / 6 blocks 355 / 340 / 336 us; eight elements a thread 379 us at best.
+// Elements of a block where that makes blocks enough; else one group per thread (512 with 8-bit moments, 2048), the shortest way
+// through.
 template <bool BITS8>
-constexpr int kThreads = BITS8 ? 64 : 256;
+constexpr int kChunk = BITS8 ? 8192 : 4096;
+// Threads of a block, and blocks per SM.  The 8-bit form at 176M parameters, sixteen elements a thread, the next group on its way:
+// one warp a block, 16 blocks 308 us (copy rate: 272); 64 threads, 8 blocks 310 to 334 us; without the loads ahead 330 us at best;
+// eight elements a thread 379 us.
 template <bool BITS8>
-constexpr int kBlocks = BITS8 ? 10 : 4;
+constexpr int kThreads = BITS8 ? 32 : 256;
+template <bool BITS8>
+constexpr int kBlocks = BITS8 ? 16 : 4;
 
 struct Entry {
   AdamTensor t;
@@ -261,27 +264,44 @@ DFB_DEVICE void step(const AdamTensor& t, const AdamHyper& h, Loaded<WK, GB, BIT
   }
 }
 
-// A chunk of one tensor.
+template <int WK, int GB, bool BITS8, bool FULL>
+DFB_DEVICE Loaded<WK, GB, BITS8> fetch(const AdamTensor& t, long long i) {
+  constexpr int E = kPer<BITS8>, WB = WK == kAdamF32 || WK == kAdamMaster ? 4 : 2, SB = BITS8 ? 1 : 4;
+  Loaded<WK, GB, BITS8> in;
+  in.w = load<WB, E, FULL>(WK == kAdamMaster ? t.extra : t.w, i, t.n);
+  if constexpr (WK == kAdamSplit) in.lo = load<2, E, FULL>(t.extra, i, t.n);
+  in.g = load<GB, E, FULL>(t.g, i, t.n);
+  in.m = load<SB, E, FULL>(t.m, i, t.n);
+  in.v = load<SB, E, FULL>(t.v, i, t.n);
+  if constexpr (BITS8) {                     // read here, written behind the shuffles of the lanes that share it
+    in.sm = FULL || i < t.n ? t.m_scale[i >> 7] : 0.f;
+    in.sv = FULL || i < t.n ? t.v_scale[i >> 7] : 0.f;
+  }
+  return in;
+}
+
+// A chunk of one tensor.  With 8-bit moments a thread's next group is on its way while it computes on this one; with fp32 moments
+// the registers for that cost more than it gains (42M parameters with a master: 249 us with, 176 us without).
 template <int WK, int GB, bool BITS8, bool FULL>
 DFB_DEVICE void chunk(const AdamTensor& t, const AdamHyper& h, long long base, int elems) {
-  constexpr int E = kPer<BITS8>;
-  constexpr int WB = WK == kAdamF32 || WK == kAdamMaster ? 4 : 2, SB = BITS8 ? 1 : 4;
-  const long long n = t.n;
+  constexpr int kGroup = kThreads<BITS8> * kPer<BITS8>;
+  long long i = base + threadIdx.x * kPer<BITS8>;
+  if constexpr (FULL && BITS8) {
+    Loaded<WK, GB, BITS8> in = fetch<WK, GB, BITS8, true>(t, i);
 #pragma unroll 1
-  for (int at = 0; at < elems; at += kThreads<BITS8> * E) {
-    const long long first = base + at, i = first + threadIdx.x * E;
-    if (!FULL && first >= n) return;         // uniform over the block: the shuffles stay whole
-    Loaded<WK, GB, BITS8> in;
-    in.w = load<WB, E, FULL>(WK == kAdamMaster ? t.extra : t.w, i, n);
-    if constexpr (WK == kAdamSplit) in.lo = load<2, E, FULL>(t.extra, i, n);
-    in.g = load<GB, E, FULL>(t.g, i, n);
-    in.m = load<SB, E, FULL>(t.m, i, n);
-    in.v = load<SB, E, FULL>(t.v, i, n);
-    if constexpr (BITS8) {                   // read here, written behind the shuffles of the lanes that share it
-      in.sm = FULL || i < n ? t.m_scale[i >> 7] : 0.f;
-      in.sv = FULL || i < n ? t.v_scale[i >> 7] : 0.f;
+    for (int left = elems - kGroup; left > 0; left -= kGroup) {
+      const Loaded<WK, GB, BITS8> next = fetch<WK, GB, BITS8, true>(t, i + kGroup);
+      step<WK, GB, BITS8, true>(t, h, in, i);
+      in = next;
+      i += kGroup;
     }
-    step<WK, GB, BITS8, FULL>(t, h, in, i);
+    step<WK, GB, BITS8, true>(t, h, in, i);
+  } else {
+#pragma unroll 1
+    for (int at = 0; at < elems && (FULL || base + at < t.n); at += kGroup, i += kGroup) {      // uniform over the block
+      Loaded<WK, GB, BITS8> in = fetch<WK, GB, BITS8, FULL>(t, i);
+      step<WK, GB, BITS8, FULL>(t, h, in, i);
+    }
   }
 }
 
@@ -307,7 +327,8 @@ int launch(const AdamTensor* t, int count, int weights, bool g_f32, bool bits8, 
   long long total = 0, blocks = 0;
   for (int i = 0; i < count; ++i) total += t[i].n;
   const int group = bits8 ? kThreads<true> * kPer<true> : kThreads<false> * kPer<false>;
-  a.chunk = total >= static_cast<long long>(num_sms) * (bits8 ? kBlocks<true> : kBlocks<false>) * kChunk ? kChunk : group;
+  const int chunk = bits8 ? kChunk<true> : kChunk<false>, resident = num_sms * (bits8 ? kBlocks<true> : kBlocks<false>);
+  a.chunk = total >= static_cast<long long>(resident) * chunk ? chunk : group;
   for (int i = 0; i < count; ++i) {
     a.e[i].t = t[i];
     a.e[i].first_block = static_cast<int>(blocks);
