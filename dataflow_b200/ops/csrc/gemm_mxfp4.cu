@@ -386,18 +386,19 @@ DFB_PTX float4 load_remote(uint32_t smem_addr, uint32_t rank) {
   return v;
 }
 
-// grid (splits * tiles of N, tiles of M), clusters of `splits` along x
+// grid (SPLITS * tiles of N, tiles of M), clusters of SPLITS along x
+template <int SPLITS>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_mxfp4_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
-                         const __grid_constant__ CUtensorMap tmap_sw, const __grid_constant__ CUtensorMap tmap_sx, Params p, int splits) {
+                         const __grid_constant__ CUtensorMap tmap_sw, const __grid_constant__ CUtensorMap tmap_sx, Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Barriers* sb = reinterpret_cast<Barriers*>(smem + STAGES * STAGE_BYTES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(ptx::cluster_ctarank());
-  const int n0 = (blockIdx.x / splits) * TM, m0 = blockIdx.y * TN;
+  const int n0 = (blockIdx.x / SPLITS) * TM, m0 = blockIdx.y * TN;
   const int tokens = min(TN, p.M - m0), mma_n = (tokens + 15) & ~15;
-  const int k_blocks = (p.K + BK - 1) / BK, per = (k_blocks + splits - 1) / splits;
+  const int k_blocks = (p.K + BK - 1) / BK, per = (k_blocks + SPLITS - 1) / SPLITS;
   const int k_lo = min(rank * per, k_blocks), k_hi = min(k_lo + per, k_blocks);
   volatile int* abort_flag = &sb->abort;
   if (threadIdx.x == 0) {
@@ -473,25 +474,31 @@ gemm_mxfp4_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __gri
   ptx::cluster_sync();
   // this CTA's share of the tokens: one warp takes a token, a lane four neighbouring outputs
   const int n = n0 + lane * 4;
-  for (int t = rank * 4 + warp; t < tokens; t += splits * 4) {
+  for (int t = rank * 4 + warp; t < tokens; t += SPLITS * 4) {
     const uint32_t at = ptx::smem_u32(part + t * TM + lane * 4);
-    float f[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int r = 0; r < splits; ++r) {
-      const float4 v = load_remote(at, r);
-      f[0] += v.x; f[1] += v.y; f[2] += v.z; f[3] += v.w;
-    }
     const long long row = m0 + t;
+    float4 v[SPLITS];                        // all of them on their way at once
+#pragma unroll
+    for (int r = 0; r < SPLITS; ++r) v[r] = load_remote(at, r);
+    float more[4] = {0.f, 0.f, 0.f, 0.f};    // bias and addend
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (n + i < p.N) {
-        if (p.bias) f[i] += bf2f(reinterpret_cast<const bf16*>(p.bias)[n + i]);
-        if (p.d_is_f32) {
-          if (p.addend) f[i] += reinterpret_cast<const float*>(p.addend)[row * p.ld_add + n + i];
-          reinterpret_cast<float*>(p.D)[row * p.ldd + n + i] = f[i];
-        } else {
-          if (p.addend) f[i] += bf2f(reinterpret_cast<const bf16*>(p.addend)[row * p.ld_add + n + i]);
-          reinterpret_cast<bf16*>(p.D)[row * p.ldd + n + i] = f2bf(f[i]);
-        }
+        if (p.bias) more[i] = bf2f(reinterpret_cast<const bf16*>(p.bias)[n + i]);
+        if (p.addend)
+          more[i] += p.d_is_f32 ? reinterpret_cast<const float*>(p.addend)[row * p.ld_add + n + i]
+                                : bf2f(reinterpret_cast<const bf16*>(p.addend)[row * p.ld_add + n + i]);
+      }
+    float f[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < SPLITS; ++r) {
+      f[0] += v[r].x; f[1] += v[r].y; f[2] += v[r].z; f[3] += v[r].w;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < p.N) {
+        if (p.d_is_f32) reinterpret_cast<float*>(p.D)[row * p.ldd + n + i] = f[i] + more[i];
+        else reinterpret_cast<bf16*>(p.D)[row * p.ldd + n + i] = f2bf(f[i] + more[i]);
       }
   }
   __syncthreads();
@@ -559,8 +566,11 @@ int gemm_mxfp4(const void* A, const void* sa, const void* B, const void* sb, voi
   const long long pair_cost = (tiles + clusters - 1) / clusters * k_blocks;
   const long long skinny_cost = (ctas * splits + num_sms - 1) / num_sms * ((k_blocks + splits - 1) / splits);
   if (skinny_cost < pair_cost && (M + skinny::TN - 1) / skinny::TN <= 65535) {
-    static std::atomic<bool> ready[64];
-    if (!configure(skinny::gemm_mxfp4_skinny_kernel, skinny::SMEM_BYTES, ready)) return -1;
+    static std::atomic<bool> ready[4][64];
+    const int which = splits == 1 ? 0 : splits == 2 ? 1 : splits == 4 ? 2 : 3;
+    auto kernel = which == 0 ? skinny::gemm_mxfp4_skinny_kernel<1> : which == 1 ? skinny::gemm_mxfp4_skinny_kernel<2>
+                : which == 2 ? skinny::gemm_mxfp4_skinny_kernel<4> : skinny::gemm_mxfp4_skinny_kernel<8>;
+    if (!configure(kernel, skinny::SMEM_BYTES, ready[which])) return -1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>((N + skinny::TM - 1) / skinny::TM) * splits, static_cast<unsigned>((M + skinny::TN - 1) / skinny::TN));
     cfg.blockDim = dim3(skinny::THREADS);
@@ -572,7 +582,7 @@ int gemm_mxfp4(const void* A, const void* sa, const void* B, const void* sb, voi
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, skinny::gemm_mxfp4_skinny_kernel, tb, ta, tsb, tsa, p, splits) == cudaSuccess ? 0 : -1;
+    return cudaLaunchKernelEx(&cfg, kernel, tb, ta, tsb, tsa, p) == cudaSuccess ? 0 : -1;
   }
   static std::atomic<bool> ready[64];
   if (!configure(gemm_mxfp4_kernel, SMEM_BYTES, ready)) return -1;
