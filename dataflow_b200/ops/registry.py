@@ -97,16 +97,11 @@ class KernelSet:
         self._table = dict(table)
         self.caps = dict(caps)
         self._sets = dict(sets or {})
+        # plain attributes: a call of a small kernel is bound by the host
+        self.__dict__.update({op: k.fn for op, k in self._table.items()}, **self._sets)
 
     def __getattr__(self, op: str):
-        if op.startswith("__"):                  # copying and pickling probe for these before the tables exist
-            raise AttributeError(op)
-        if op in self._sets:
-            return self._sets[op]
-        try:
-            return self._table[op].fn
-        except KeyError:
-            raise AttributeError(f"no kernel registered for op {op!r}") from None
+        raise AttributeError(f"no kernel registered for op {op!r}")
 
     def impl(self, op: str) -> KernelImpl:
         return self._table[op]
