@@ -557,15 +557,18 @@ int gemm_mxfp4(const void* A, const void* sa, const void* B, const void* sb, voi
   p.ldd = ldd; p.ld_add = ld_add; p.d_is_f32 = d_f32;
   p.group_m = 16;
   p.tma_epi = tma_epi;
-  // The pair kernel takes `waves` rounds of k_blocks stages over the pairs.  Where its tiles leave SMs idle the skinny kernel
-  // may need fewer stages per CTA; a stage costs about the same in both (it is the loads that take the time).
+  // Stages that a CTA goes through one after the other: `pair` in the pair kernel, `few` in the skinny one, whose stages take as
+  // long for a quarter of the outputs, and whose sums pass through shared memory.  It is taken where it halves the stages of a call
+  // with at most 256 tokens, or does not lengthen them with at most 64.  us of the pair / skinny kernel, tokens x N x K: 17 x 4096 x
+  // 4096 10.5 / 6.2, 128: 10.8 / 8.1, 256: 11.1 / 10.4, 512: 11.3 / 12.6; 64 x 14336 x 4096 13.2 / 11.7; 300 x 14336 x 4096
+  // 18.7 / 30.1; 1024 x 1024 x 1024 7.4 / 8.5.
   const int clusters = num_sms / 2;
   const long long ctas = (N + skinny::TM - 1) / skinny::TM * ((M + skinny::TN - 1) / skinny::TN);
   int splits = 1;
   while (splits < 8 && ctas * splits * 2 <= num_sms && splits * 2 <= k_blocks) splits *= 2;
-  const long long pair_cost = (tiles + clusters - 1) / clusters * k_blocks;
-  const long long skinny_cost = (ctas * splits + num_sms - 1) / num_sms * ((k_blocks + splits - 1) / splits);
-  if (skinny_cost < pair_cost && (M + skinny::TN - 1) / skinny::TN <= 65535) {
+  const long long pair = (tiles + clusters - 1) / clusters * k_blocks;
+  const long long few = (ctas * splits + num_sms - 1) / num_sms * ((k_blocks + splits - 1) / splits);
+  if (M <= 64 ? few <= pair : M <= 256 && 2 * few <= pair) {
     static std::atomic<bool> ready[4][64];
     const int which = splits == 1 ? 0 : splits == 2 ? 1 : splits == 4 ? 2 : 3;
     auto kernel = which == 0 ? skinny::gemm_mxfp4_skinny_kernel<1> : which == 1 ? skinny::gemm_mxfp4_skinny_kernel<2>

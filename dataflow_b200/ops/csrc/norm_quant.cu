@@ -101,7 +101,7 @@ struct NormArgs {
 // (one row per block left a gap between a row's loads and the last block's stores: 88 us at 16384 x 4096, now 80); the gain stays
 // in registers.  A block takes max(1, 128 / T) rows at a time.
 template <bool MX, bool RES, int T, int VPT>
-__global__ void __launch_bounds__(T < 128 ? 128 : T, T <= 256 ? 1024 / (T < 128 ? 128 : T) : 1)
+__global__ void __launch_bounds__(T < 128 ? 128 : T, VPT <= 2 ? 1024 / (T < 128 ? 128 : T) : 1)
 rmsnorm_quant_kernel(const __grid_constant__ NormArgs a) {
   __shared__ float part[2][2][T / 32];             // [sum | max][parity of the row]: the next row's writes never meet this row's reads
   static_assert(T == 32 || T >= 128, "a row is one warp (no barrier) or a whole block");
@@ -240,13 +240,17 @@ int launch(const NormArgs& a, int num_sms, cudaStream_t s) {
     const long long need = (rows + rows_per_block - 1) / rows_per_block, fit = static_cast<long long>(num_sms) * (1024 / threads);
     kernel<<<static_cast<unsigned>(need < fit ? need : fit), threads, 0, s>>>(a);
   };
+  // Threads of a row by its width, measured in us with the residual into 8 bits (16384 rows; 8192 and 4096 of the last two):
+  //    256 columns: a warp 7, 128 threads 16         512: 13, 19        1024: 24, 25, 256 threads 38
+  //   2048: 128 threads 39, 256 48                  4096: 256 80, 512 104 or more
+  //   8192: 512 of two vectors 95, of four 143, 1024 137, unheld 141    16384: 512 of four 116, 1024 129, unheld 131
   if (nvec <= 32) go(rmsnorm_quant_kernel<MX, RES, 32, 1>, 128, 4);
   else if (nvec <= 64) go(rmsnorm_quant_kernel<MX, RES, 32, 2>, 128, 4);
   else if (nvec <= 128) go(rmsnorm_quant_kernel<MX, RES, 32, 4>, 128, 4);
   else if (nvec <= 256) go(rmsnorm_quant_kernel<MX, RES, 128, 2>, 128, 1);
   else if (nvec <= 512) go(rmsnorm_quant_kernel<MX, RES, 256, 2>, 256, 1);
   else if (nvec <= 1024) go(rmsnorm_quant_kernel<MX, RES, 512, 2>, 512, 1);
-  else if (nvec <= 2048) go(rmsnorm_quant_kernel<MX, RES, 1024, 2>, 1024, 1);
+  else if (nvec <= 2048) go(rmsnorm_quant_kernel<MX, RES, 512, 4>, 512, 1);
   else rmsnorm_quant_wide_kernel<MX, RES><<<static_cast<unsigned>(rows), 512, 0, s>>>(a);
   return cudaGetLastError() == cudaSuccess ? 0 : -1;
 }
