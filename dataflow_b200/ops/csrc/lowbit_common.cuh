@@ -60,10 +60,11 @@ DFB_DEVICE float mx_amax8(const float* f) {
   for (int i = 1; i < 8; ++i) a = max_nan(a, fabsf(f[i]));
   return a;
 }
-// over the four neighbouring lanes that hold a block
-DFB_DEVICE float mx_amax4lanes(float a) {
-  a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));
-  return max_nan(a, __shfl_xor_sync(0xffffffffu, a, 2));
+// over the four (eight elements a lane) or two (sixteen) neighbouring lanes that hold a block
+template <int LANES>
+DFB_DEVICE float mx_amax_lanes(float a) {
+  if constexpr (LANES == 4) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, 2));
+  return max_nan(a, __shfl_xor_sync(0xffffffffu, a, 1));
 }
 // f *= 2^k in pairs, then the codes
 DFB_DEVICE uint32_t mx_pack8(const float* f);
@@ -108,11 +109,22 @@ DFB_DEVICE void mx_unpack8(uint32_t c, float* f) {
   }
 }
 
-// Scale bytes of four neighbouring blocks (lanes 0-3, 4-7, 8-11, 12-15 of a half warp hold one each) as the tile's word.
+// Scale bytes of four neighbouring blocks, LANES lanes to a block, as the tile's word.
+template <int LANES>
 DFB_DEVICE uint32_t mx_scale_word(uint32_t byte) {
-  uint32_t w = byte << (8 * ((threadIdx.x >> 2) & 3));
-  w |= __shfl_xor_sync(0xffffffffu, w, 4);
-  return w | __shfl_xor_sync(0xffffffffu, w, 8);
+  uint32_t w = byte << (8 * ((threadIdx.x / LANES) & 3));
+  w |= __shfl_xor_sync(0xffffffffu, w, LANES);
+  return w | __shfl_xor_sync(0xffffffffu, w, 2 * LANES);
+}
+
+// 32 bytes in one access (aligned to them)
+DFB_DEVICE void load32(const void* p, uint32_t* u) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]) : "l"(p) : "memory");
+}
+DFB_DEVICE void store32(void* p, const uint32_t* u) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               :: "l"(p), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]) : "memory");
 }
 
 // two e4m3 codes: a in the low byte

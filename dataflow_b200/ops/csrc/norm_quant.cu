@@ -65,8 +65,8 @@ DFB_DEVICE void scaled(const bf16x8& h, const bf16x8& w, float r, float* f) {
 template <bool MX>
 DFB_DEVICE void emit(const float* f, float inv, bool on, uint8_t* q, uint8_t* tile, int v) {
   if constexpr (MX) {
-    const uint32_t sb = mx_scale_byte(mx_amax4lanes(mx_amax8(f)));
-    const uint32_t word = mx_scale_word(sb);          // columns that do not exist count as zero blocks
+    const uint32_t sb = mx_scale_byte(mx_amax_lanes<4>(mx_amax8(f)));
+    const uint32_t word = mx_scale_word<4>(sb);          // columns that do not exist count as zero blocks
     if (on) {
       *reinterpret_cast<uint32_t*>(q + v * 4) = mx_scale_pack8(f, mx_scale_inv(sb));
       if ((v & 15) == 0) *reinterpret_cast<uint32_t*>(tile + (v >> 4) * 512) = word;

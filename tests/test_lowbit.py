@@ -134,6 +134,19 @@ def test_quant_takes_strided_and_offset_rows(dev):
         assert torch.equal(q, q2) and torch.equal(s, s2)
 
 
+@pytest.mark.gpu
+def test_more_rows_than_a_grid_axis_holds():
+    """Both walks go out in slices there; rows behind the first slice are what a call on them alone gives."""
+    k = lane("cuda")
+    rows = 2_200_013
+    x = torch.randn(rows, 32, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(BF)
+    q, s = k.quant_mxfp4(x)
+    y = k.dequant_mxfp4(q, s)
+    for a, b in ((0, 300), (2_096_896, 2_097_280), (rows - 141, rows)):
+        q1, s1 = k.quant_mxfp4(x[a:b])
+        assert torch.equal(q[a:b], q1) and torch.equal(y[a:b], k.dequant_mxfp4(q1, s1))
+
+
 @pytest.mark.parametrize("dev", LANES)
 def test_no_rows(dev):
     k = lane(dev)
