@@ -312,6 +312,19 @@ def test_norm_layouts_and_edges(dev):
     got = k.rmsnorm_fp8(x, w, residual=r)
     for a, b in zip(want, got):
         assert torch.equal(a.view(U8), b.contiguous().view(U8))
+    # rows that start on 32 bytes, on 16 only, and widths that are not 16s: the same numbers
+    for cols, off in ((320, 8), (320, 16), (2080, 8), (4128, 8), (8224, 8), (16416, 8), (328, 0), (1032, 8), (2056, 0)):
+        big = rnd(dev, 3, cols + 64, seed=cols)
+        gain = (1 + 0.1 * rnd(dev, cols + 8, seed=3, dtype=F32)).to(BF)
+        xv, rv, gv = big[:, off:off + cols], big[:, 48:48 + cols], gain[:cols]
+        for fn in (k.rmsnorm_fp8, k.rmsnorm_mxfp4) if cols % 32 == 0 else (k.rmsnorm_fp8,):
+            for g_, w_ in zip(fn(xv, gv, residual=rv), fn(xv.contiguous(), gv.clone(), residual=rv.contiguous())):
+                if g_.dtype == F32:               # the threads of a row differ between the forms, and with them the sum's order
+                    assert ((g_ - w_).abs() <= (cols + 8) * U * w_.abs()).all()
+                elif g_.dtype == BF:
+                    assert torch.equal(g_, w_)
+                else:
+                    assert (g_.contiguous().view(U8) != w_.view(U8)).double().mean() < 1e-2
     # the sum may replace the residual stream in place, as a view of a wider buffer
     buf = wide.clone()
     q, s, h, rstd = k.rmsnorm_fp8(x, w, residual=buf[:, 80:144], h_out=buf[:, 80:144])
