@@ -8,7 +8,7 @@
 // index, seed).  A positive r keeps at least the smallest code.  The update itself uses the unrounded moments.
 //
 // The kernel moves 10 bytes per element with 8-bit moments (28 with fp32 moments and a master) and is bound by memory
-// (8 bits: 0.89 of the copy rate at 218M parameters, 379 us, with the arithmetic close behind: 45 instructions an element; 32 bits:
+// (8 bits: 0.9 of the copy rate at 218M parameters, 373 us, with the arithmetic close behind: 45 instructions an element; 32 bits:
 // 1.0).  A block takes consecutive elements of one tensor, a thread eight or (8-bit moments) sixteen of them, so that eight lanes
 // share a scale.  Tensors travel as a table in the kernel's parameters (no copy, no device-side table that a captured graph would share); a block finds its tensor
 // by bisection.
@@ -23,8 +23,8 @@ namespace {
 // 42M 86 / 90 us; fp32, 4096 / 2048: 1M 5.0 / 4.7 us, 42M 138 / 135 us.
 constexpr int kChunk = 8192;
 // Threads of a block, and blocks per SM.  The 8-bit form at 176M parameters, sixteen elements a thread, the next group on its way:
-// one warp a block, 16 blocks 308 us (copy rate: 272); 64 threads, 8 blocks 310 to 334 us; without the loads ahead 330 us at best;
-// eight elements a thread 379 us.
+// one warp a block, 16 blocks 304 us (copy rate: 272), 18 blocks 363; 64 threads, 8 blocks 303 to 309 us; without the loads ahead 330
+// at best; eight elements a thread 379.
 template <bool BITS8>
 constexpr int kThreads = BITS8 ? 32 : 256;
 template <bool BITS8>
@@ -79,14 +79,19 @@ DFB_DEVICE float dither_any(float y, uint32_t rnd16) {
   return copysignf(t, y);
 }
 
-// Eight elements as they lie in memory; a load that may not be whole (FULL false) goes element by element, zeros past n.  The two
-// forms are chosen once per block, so that a thread's loads stand one behind the other without a branch between.
+// A thread's elements as they lie in memory.  How they are fetched is chosen once per block, so that the loads stand one behind
+// the other without a branch between: 32 bytes at a time with 8-bit moments where every operand of the tensor starts on 32 (176M parameters
+// 304 us; by 16 bytes 309 to 319; with fp32 moments both at the copy rate), 16 bytes where on 16, else element by element, zeros past n.
+enum Fetch { kElements, k16Bytes, k32Bytes };
 template <int BYTES, int E>
-struct alignas(BYTES * E >= 16 ? 16 : 8) Raw { uint32_t u[BYTES * E / 4]; };      // E elements of BYTES bytes, 16 bytes at least
-template <int BYTES, int E, bool FULL>
+struct alignas(BYTES * E >= 16 ? 16 : 8) Raw { uint32_t u[BYTES * E / 4]; };      // E elements of BYTES bytes
+template <int BYTES, int E, int HOW>
 DFB_DEVICE Raw<BYTES, E> load(const void* p, long long i, long long n) {
   Raw<BYTES, E> r;
-  if constexpr (FULL) {
+  if constexpr (HOW == k32Bytes && BYTES * E % 32 == 0) {
+#pragma unroll
+    for (int k = 0; k < BYTES * E / 32; ++k) load32(static_cast<const char*>(p) + i * BYTES + k * 32, r.u + k * 8);
+  } else if constexpr (HOW != kElements) {
     r = *reinterpret_cast<const Raw<BYTES, E>*>(static_cast<const char*>(p) + i * BYTES);
   } else {
 #pragma unroll
@@ -101,9 +106,12 @@ DFB_DEVICE Raw<BYTES, E> load(const void* p, long long i, long long n) {
   }
   return r;
 }
-template <int BYTES, int E, bool FULL>
+template <int BYTES, int E, int HOW>
 DFB_DEVICE void store(void* p, long long i, long long n, const Raw<BYTES, E>& r) {
-  if constexpr (FULL) {
+  if constexpr (HOW == k32Bytes && BYTES * E % 32 == 0) {
+#pragma unroll
+    for (int k = 0; k < BYTES * E / 32; ++k) store32(static_cast<char*>(p) + i * BYTES + k * 32, r.u + k * 8);
+  } else if constexpr (HOW != kElements) {
     *reinterpret_cast<Raw<BYTES, E>*>(static_cast<char*>(p) + i * BYTES) = r;
   } else {
 #pragma unroll
@@ -152,7 +160,7 @@ struct Loaded {
 
 // The elements of one thread.  Products and sums in front of the 8-bit rounding are rounded one by one (a sum is a fused product
 // with a factor of one that the compiler does not know), so a state has the same codes here and in the plain-torch lane.
-template <int WK, int GB, bool BITS8, bool FULL>
+template <int WK, int GB, bool BITS8, int HOW>
 DFB_DEVICE void step(const AdamTensor& t, const AdamHyper& h, Loaded<WK, GB, BITS8>& in, long long i) {
   constexpr int E = kPer<BITS8>, P = E / 2;
   const long long n = t.n;
@@ -178,7 +186,7 @@ DFB_DEVICE void step(const AdamTensor& t, const AdamHyper& h, Loaded<WK, GB, BIT
       ar = fmaxf(ar, fmaxf(r[j].x, r[j].y));
     }
     const float sm = fmaxf(__fmul_rn(max_lanes<128 / E>(am), 1.f / kE4M3Top), kMinScale), sr = fmaxf(__fmul_rn(max_lanes<128 / E>(ar), 1.f / kE4M3Top), kMinScale);
-    if ((FULL || i < n) && (threadIdx.x & (128 / E - 1)) == 0) {
+    if ((HOW != kElements || i < n) && (threadIdx.x & (128 / E - 1)) == 0) {
       t.m_scale[i >> 7] = sm;
       t.v_scale[i >> 7] = sr;
     }
@@ -228,8 +236,8 @@ DFB_DEVICE void step(const AdamTensor& t, const AdamHyper& h, Loaded<WK, GB, BIT
       r[j] = make_float2(sqrtf(r[j].x), sqrtf(r[j].y));
     }
   }
-  store<BITS8 ? 1 : 4, E, FULL>(t.m, i, n, in.m);
-  store<BITS8 ? 1 : 4, E, FULL>(t.v, i, n, in.v);
+  store<BITS8 ? 1 : 4, E, HOW>(t.m, i, n, in.m);
+  store<BITS8 ? 1 : 4, E, HOW>(t.v, i, n, in.v);
 #pragma unroll
   for (int j = 0; j < P; ++j) {
     const float2 den = fma2(r[j], both(h.inv_sqrt_bc2), both(h.eps));
@@ -245,62 +253,62 @@ DFB_DEVICE void step(const AdamTensor& t, const AdamHyper& h, Loaded<WK, GB, BIT
       hi.u[j] = ((a + 0x8000u) >> 16) | ((b + 0x8000u) & 0xffff0000u);
       in.lo.u[j] = (a & 0xffffu) | (b << 16);
     }
-    store<2, E, FULL>(t.w, i, n, hi);
-    store<2, E, FULL>(t.extra, i, n, in.lo);
+    store<2, E, HOW>(t.w, i, n, hi);
+    store<2, E, HOW>(t.extra, i, n, in.lo);
   } else if constexpr (WK == kAdamF32) {
 #pragma unroll
     for (int j = 0; j < P; ++j) set_pair(in.w, j, w[j]);
-    store<4, E, FULL>(t.w, i, n, in.w);
+    store<4, E, HOW>(t.w, i, n, in.w);
   } else {
     Raw<2, E> out;
 #pragma unroll
     for (int j = 0; j < P; ++j) set_pair(out, j, w[j]);
-    store<2, E, FULL>(t.w, i, n, out);
+    store<2, E, HOW>(t.w, i, n, out);
     if constexpr (WK == kAdamMaster) {
 #pragma unroll
       for (int j = 0; j < P; ++j) set_pair(in.w, j, w[j]);
-      store<4, E, FULL>(t.extra, i, n, in.w);
+      store<4, E, HOW>(t.extra, i, n, in.w);
     }
   }
 }
 
-template <int WK, int GB, bool BITS8, bool FULL>
+template <int WK, int GB, bool BITS8, int HOW>
 DFB_DEVICE Loaded<WK, GB, BITS8> fetch(const AdamTensor& t, long long i) {
   constexpr int E = kPer<BITS8>, WB = WK == kAdamF32 || WK == kAdamMaster ? 4 : 2, SB = BITS8 ? 1 : 4;
   Loaded<WK, GB, BITS8> in;
-  in.w = load<WB, E, FULL>(WK == kAdamMaster ? t.extra : t.w, i, t.n);
-  if constexpr (WK == kAdamSplit) in.lo = load<2, E, FULL>(t.extra, i, t.n);
-  in.g = load<GB, E, FULL>(t.g, i, t.n);
-  in.m = load<SB, E, FULL>(t.m, i, t.n);
-  in.v = load<SB, E, FULL>(t.v, i, t.n);
+  in.w = load<WB, E, HOW>(WK == kAdamMaster ? t.extra : t.w, i, t.n);
+  if constexpr (WK == kAdamSplit) in.lo = load<2, E, HOW>(t.extra, i, t.n);
+  in.g = load<GB, E, HOW>(t.g, i, t.n);
+  in.m = load<SB, E, HOW>(t.m, i, t.n);
+  in.v = load<SB, E, HOW>(t.v, i, t.n);
   if constexpr (BITS8) {                     // read here, written behind the shuffles of the lanes that share it
-    in.sm = FULL || i < t.n ? t.m_scale[i >> 7] : 0.f;
-    in.sv = FULL || i < t.n ? t.v_scale[i >> 7] : 0.f;
+    in.sm = HOW != kElements || i < t.n ? t.m_scale[i >> 7] : 0.f;
+    in.sv = HOW != kElements || i < t.n ? t.v_scale[i >> 7] : 0.f;
   }
   return in;
 }
 
 // A chunk of one tensor.  With 8-bit moments a thread's next group is on its way while it computes on this one; with fp32 moments
 // the registers for that cost more than it gains (42M parameters with a master: 249 us with, 176 us without).
-template <int WK, int GB, bool BITS8, bool FULL>
+template <int WK, int GB, bool BITS8, int HOW>
 DFB_DEVICE void chunk(const AdamTensor& t, const AdamHyper& h, long long base, int elems) {
   constexpr int kGroup = kThreads<BITS8> * kPer<BITS8>;
   long long i = base + threadIdx.x * kPer<BITS8>;
-  if constexpr (FULL && BITS8) {
-    Loaded<WK, GB, BITS8> in = fetch<WK, GB, BITS8, true>(t, i);
+  if constexpr (HOW != kElements && BITS8) {
+    Loaded<WK, GB, BITS8> in = fetch<WK, GB, BITS8, HOW>(t, i);
 #pragma unroll 1
     for (int left = elems - kGroup; left > 0; left -= kGroup) {
-      const Loaded<WK, GB, BITS8> next = fetch<WK, GB, BITS8, true>(t, i + kGroup);
-      step<WK, GB, BITS8, true>(t, h, in, i);
+      const Loaded<WK, GB, BITS8> next = fetch<WK, GB, BITS8, HOW>(t, i + kGroup);
+      step<WK, GB, BITS8, HOW>(t, h, in, i);
       in = next;
       i += kGroup;
     }
-    step<WK, GB, BITS8, true>(t, h, in, i);
+    step<WK, GB, BITS8, HOW>(t, h, in, i);
   } else {
 #pragma unroll 1
-    for (int at = 0; at < elems && (FULL || base + at < t.n); at += kGroup, i += kGroup) {      // uniform over the block
-      Loaded<WK, GB, BITS8> in = fetch<WK, GB, BITS8, FULL>(t, i);
-      step<WK, GB, BITS8, FULL>(t, h, in, i);
+    for (int at = 0; at < elems && (HOW != kElements || base + at < t.n); at += kGroup, i += kGroup) {      // uniform over the block
+      Loaded<WK, GB, BITS8> in = fetch<WK, GB, BITS8, HOW>(t, i);
+      step<WK, GB, BITS8, HOW>(t, h, in, i);
     }
   }
 }
@@ -315,10 +323,18 @@ __global__ void __launch_bounds__(kThreads<BITS8>, kBlocks<BITS8>) adamw_multi_k
   }
   const AdamTensor& t = a.e[lo].t;
   const long long base = static_cast<long long>(blockIdx.x - a.e[lo].first_block) * a.chunk;
-  const bool vec = ((reinterpret_cast<uintptr_t>(t.w) | reinterpret_cast<uintptr_t>(t.g) | reinterpret_cast<uintptr_t>(t.extra)) & 15) == 0 &&
-                   ((reinterpret_cast<uintptr_t>(t.m) | reinterpret_cast<uintptr_t>(t.v)) & 15) == 0;
-  if (vec && base + a.chunk <= t.n) chunk<WK, GB, BITS8, true>(t, a.h, base, a.chunk);
-  else chunk<WK, GB, BITS8, false>(t, a.h, base, a.chunk);
+  // the codes of 8-bit moments are 16 bytes a thread at most
+  const uintptr_t wide = reinterpret_cast<uintptr_t>(t.w) | reinterpret_cast<uintptr_t>(t.g) | reinterpret_cast<uintptr_t>(t.extra);
+  const uintptr_t state = reinterpret_cast<uintptr_t>(t.m) | reinterpret_cast<uintptr_t>(t.v);
+  const bool whole = base + a.chunk <= t.n && (state & 15) == 0;
+  if constexpr (BITS8) {
+    if (whole && (wide & 31) == 0) {
+      chunk<WK, GB, BITS8, k32Bytes>(t, a.h, base, a.chunk);
+      return;
+    }
+  }
+  if (whole && (wide & 15) == 0) chunk<WK, GB, BITS8, k16Bytes>(t, a.h, base, a.chunk);
+  else chunk<WK, GB, BITS8, kElements>(t, a.h, base, a.chunk);
 }
 
 template <int NT>

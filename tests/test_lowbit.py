@@ -427,7 +427,7 @@ def dither_ref(y, rnd16):
 @pytest.mark.parametrize("bits", [8, 32])
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("gdt", [BF, F32], ids=["gbf16", "gfp32"])
-@pytest.mark.parametrize("offset", [0, 1], ids=["aligned", "odd"])
+@pytest.mark.parametrize("offset", [0, 1, 8, 16], ids=["aligned", "odd", "by8", "by16"])
 def test_adamw(dev, bits, form, gdt, offset):
     k = lane(dev)
     sizes = [1, 127, 128, 129, 0, 4096, 4097, 10000, 33]
