@@ -183,6 +183,8 @@ def test_product(dev, out, M, N, K):
     assert y.dtype == out and y.shape == (M, N)
     bound = product_bound(A, B, K, out)
     assert ((y.double() - A @ B.t()).abs() <= bound).all()
+    if dev == "cuda":
+        assert native().gemm_mxfp4_last_error() == 0            # no bounded wait ran out
     add, bias = rnd(dev, M, N, seed=5, dtype=out), rnd(dev, N, seed=6)
     z = k.linear_mxfp4(*a, *b, add=add, bias=bias, out_dtype=out)
     want = A @ B.t() + add.double() + bias.double()
@@ -709,12 +711,12 @@ def test_a_training_step_in_narrow_formats(dev):
         assert ((t.double() - w1).abs() <= half_step(BF) * w1.abs() * (1 + 1e-6) + 64 * U * ((w1 - w0).abs() + w0.abs())).all()
 
 
-def _trainer_losses(dev, steps=3, hyper=None, lower=None, budget=None, **over):
+def _trainer_losses(dev, steps=3, hyper=None, lower=None, budget=None, family="llama3", **over):
     import dataclasses
     from dataflow_b200.models.families import resolve_family
     from dataflow_b200.run.driver import Trainer, synthetic_rounds
-    cfg = dataclasses.replace(resolve_family("llama3").presets["tiny"](), **over)
-    tr = Trainer("llama3", cfg, budget_gib=budget, device=None if dev == "cpu" else 0, hyper={"lr": 3e-3, **(hyper or {})}, seed=3,
+    cfg = dataclasses.replace(resolve_family(family).presets["tiny"](), **over)
+    tr = Trainer(family, cfg, budget_gib=budget, device=None if dev == "cpu" else 0, hyper={"lr": 3e-3, **(hyper or {})}, seed=3,
                  **({"lower_kwargs": lower} if lower else {}))
     out = [tr.step(synthetic_rounds(cfg, tr.rounds, tr.T, 64, 11, s)) for s in range(steps)]
     tr.close()
@@ -722,12 +724,22 @@ def _trainer_losses(dev, steps=3, hyper=None, lower=None, budget=None, **over):
 
 
 @pytest.mark.parametrize("dev", LANES)
-def test_llama_block_in_4_bits(dev):
-    base, got = _trainer_losses(dev), _trainer_losses(dev, hyper={"linear_precision": "mxfp4"})
+@pytest.mark.parametrize("family", ["llama3", "qwen3", "olmoe"])
+def test_llama_like_blocks_in_4_bits(dev, family):
+    """Dense blocks, blocks with q / k norms, and a mixture-of-experts MLP behind 4-bit attention projections."""
+    base, got = _trainer_losses(dev, family=family), _trainer_losses(dev, family=family, hyper={"linear_precision": "mxfp4"})
     assert base != got and all(math.isfinite(v) for v in got)
     for level in (1, 2):                                        # recomputed context comes from the same codes
-        again = _trainer_losses(dev, hyper={"linear_precision": "mxfp4"}, lower={"recompute_levels": {0: level, 1: level}})
+        again = _trainer_losses(dev, family=family, hyper={"linear_precision": "mxfp4"}, lower={"recompute_levels": {0: level, 1: level}})
         assert again == got
+
+
+def test_reference_form_family_in_4_bits():
+    """The twin runs the same forms, so both quantise; the engine and the twin stay together."""
+    from dataflow_b200.testing.family_gate import run_pair
+    base = run_pair("dsv32", steps=3)["engine"]
+    low = run_pair("dsv32", steps=3, overrides={"linear_precision": "mxfp4"})
+    assert low["engine"] != base and low["max_loss_rel"] < 1e-3
 
 
 @pytest.mark.parametrize("dev", LANES)
