@@ -849,3 +849,53 @@ def test_another_stream_and_a_captured_graph():
     for n in st:
         for s, t in zip(st[n], ref[n]):
             assert torch.equal(s.view(U8), t.view(U8))
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Matrices and a tensor of more than 2^31 elements: their last rows are what a call on those rows alone gives."""
+    K = lane("cuda")
+    g = torch.Generator(device="cuda").manual_seed(5)
+    rows, cols = 262_200, 8224                                   # 2.16e9 elements
+    x = torch.empty(rows, cols, dtype=BF, device="cuda")
+    for i in range(0, rows, 65536):
+        x[i:i + 65536] = torch.randn(min(65536, rows - i), cols, device="cuda", generator=g).to(BF)
+    w = (1 + 0.1 * rnd("cuda", cols, seed=1, dtype=F32)).to(BF)
+    tail = slice(rows - 77, rows)
+    q, s, h, r = K.rmsnorm_fp8(x, w, residual=x)
+    q1, s1, h1, r1 = K.rmsnorm_fp8(x[tail], w, residual=x[tail])
+    assert torch.equal(q[tail].view(U8), q1.view(U8)) and torch.equal(s[tail], s1) and torch.equal(h[tail], h1) and torch.equal(r[tail], r1)
+    del q, h
+    for fn in (K.quant_mxfp4, lambda t: K.rmsnorm_mxfp4(t, w)[:2]):
+        q, s = fn(x)
+        q1, s1 = fn(x[tail])
+        assert torch.equal(q[tail], q1) and torch.equal(K.dequant_mxfp4(q, s)[tail], K.dequant_mxfp4(q1, s1))
+    del q, s
+    xt = x.view(-1)[:8224 * 262_144].view(8224, 262_144)         # stored (K, rows)
+    q, s = K.quant_mxfp4(xt, transpose=True)
+    q1, s1 = K.quant_mxfp4(xt[:, -60:].contiguous(), transpose=True)
+    assert torch.equal(q[-60:], q1)
+    del q, s, xt, x
+    a, b = K.quant_mxfp4(rnd("cuda", 46_400, 32)), K.quant_mxfp4(rnd("cuda", 46_400, 32, seed=1))
+    y = K.linear_mxfp4(*a, *b)                                   # 2.15e9 results
+    a1 = K.quant_mxfp4(K.dequant_mxfp4(*a)[-50:])
+    assert torch.equal(y[-50:], K.linear_mxfp4(*a1, *b))
+    del y
+    n, k = 2 ** 31 + 1024 + 37, 1024 + 37
+    for bits in (8, 32):
+        ws, gs = torch.zeros(n, dtype=BF, device="cuda"), torch.zeros(n, dtype=BF, device="cuda")
+        ws[-k:], gs[-k:] = rnd("cuda", k, seed=2), rnd("cuda", k, seed=3)
+        mk = lambda c: torch.zeros(c, dtype=U8, device="cuda").view(F8) if bits == 8 else torch.zeros(c, device="cuda")
+        sc = lambda c: [torch.zeros(-(-c // 128), device="cuda")] if bits == 8 else None
+        one = [t[-k:].clone() for t in (ws, gs)]
+        m, v, ms, vs, m1, v1, ms1, vs1 = mk(n), mk(n), sc(n), sc(n), mk(k), mk(k), sc(k), sc(k)
+        K.adamw_multi_step([ws], [gs], [m], [v], 1e-2, m_scales=ms, v_scales=vs)
+        K.adamw_multi_step([one[0]], [one[1]], [m1], [v1], 1e-2, m_scales=ms1, v_scales=vs1)
+        assert torch.equal(ws[-k:], one[0])
+        if bits == 8:                                            # the random bits go by the index, the scales do not
+            assert torch.equal(ms[0][-9:], ms1[0]) and torch.equal(vs[0][-9:], vs1[0])
+            up = lambda q, s: q[-k:].float() * s[0][-9:].repeat_interleave(128)[:k]
+            assert ((up(m, ms) - up(m1, ms1)).abs() <= 0.125 * up(m1, ms1).abs() + ms1[0].max() * 2 ** -9).all()
+        else:
+            assert torch.equal(m[-k:], m1) and torch.equal(v[-k:], v1)
+        del ws, gs, m, v
