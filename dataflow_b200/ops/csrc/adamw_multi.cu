@@ -7,11 +7,11 @@
 // of e4m3's 6 to 12 % spacing, so rounding to nearest would never let it fall again.  The random bits are a hash of (element
 // index, seed).  A positive r keeps at least the smallest code.  The update itself uses the unrounded moments.
 //
-// The kernel moves 10 bytes per element with 8-bit moments (28 with fp32 moments and a master) and is bound by memory
-// (8 bits: 0.9 of the copy rate at 218M parameters, 373 us, with the arithmetic close behind: 45 instructions an element; 32 bits:
-// 1.0).  A block takes consecutive elements of one tensor, a thread eight or (8-bit moments) sixteen of them, so that eight lanes
-// share a scale.  Tensors travel as a table in the kernel's parameters (no copy, no device-side table that a captured graph would share); a block finds its tensor
-// by bisection.
+// The kernel moves 10 bytes per element with 8-bit moments (28 with fp32 moments and a master) and is bound by memory: 8 bits 372 us
+// at 218M parameters, 0.9 of the copy rate with the arithmetic close behind (45 instructions an element, issue slots 73 % busy);
+// 32 bits 175 us at 42M, the copy rate.  A block takes consecutive elements of one tensor, a thread eight or (8-bit moments) sixteen
+// of them, so that eight lanes share a scale.  Tensors travel as a table in the kernel's parameters (no copy, no device-side table
+// that a captured graph would share); a block finds its tensor by bisection.
 #include "lowbit.h"
 #include "lowbit_common.cuh"
 
@@ -80,8 +80,9 @@ DFB_DEVICE float dither_any(float y, uint32_t rnd16) {
 }
 
 // A thread's elements as they lie in memory.  How they are fetched is chosen once per block, so that the loads stand one behind
-// the other without a branch between: 32 bytes at a time with 8-bit moments where every operand of the tensor starts on 32 (176M parameters
-// 304 us; by 16 bytes 309 to 319; with fp32 moments both at the copy rate), 16 bytes where on 16, else element by element, zeros past n.
+// the other without a branch between: 32 bytes at a time with 8-bit moments where every operand of the tensor starts on 32
+// (176M parameters 304 us; by 16 bytes 309 to 319; with fp32 moments both at the copy rate), 16 bytes where on 16, else element by
+// element with zeros past n.
 enum Fetch { kElements, k16Bytes, k32Bytes };
 template <int BYTES, int E>
 struct alignas(BYTES * E >= 16 ? 16 : 8) Raw { uint32_t u[BYTES * E / 4]; };      // E elements of BYTES bytes
@@ -185,7 +186,8 @@ DFB_DEVICE void step(const AdamTensor& t, const AdamHyper& h, Loaded<WK, GB, BIT
       am = fmaxf(am, fmaxf(fabsf(m[j].x), fabsf(m[j].y)));
       ar = fmaxf(ar, fmaxf(r[j].x, r[j].y));
     }
-    const float sm = fmaxf(__fmul_rn(max_lanes<128 / E>(am), 1.f / kE4M3Top), kMinScale), sr = fmaxf(__fmul_rn(max_lanes<128 / E>(ar), 1.f / kE4M3Top), kMinScale);
+    const float sm = fmaxf(__fmul_rn(max_lanes<128 / E>(am), 1.f / kE4M3Top), kMinScale);
+    const float sr = fmaxf(__fmul_rn(max_lanes<128 / E>(ar), 1.f / kE4M3Top), kMinScale);
     if ((HOW != kElements || i < n) && (threadIdx.x & (128 / E - 1)) == 0) {
       t.m_scale[i >> 7] = sm;
       t.v_scale[i >> 7] = sr;

@@ -14,6 +14,11 @@
 // The accumulators overlap by 64 columns instead: [0, 256) and [192, 448).  The epilogue drains the shared columns first and
 // then lets the next tile's MMAs begin, so all but that quarter of the epilogue stays hidden behind the main loop.
 // Rows and blocks past the operands read as zero codes with zero scale bytes.  Every wait is bounded.
+//
+// 8192 x 28672 x 4096: 356 us alone (5.4 PFLOP/s), 409 us back to back (4.7: the power cap); 8192 x 8192 x 16384 6.35 PFLOP/s, 0.96
+// of four times the library's bf16 rate.  A stage takes about 700 cycles instead of the MMA's 512: 35 KB arrive in shared memory and
+// 32 KB are read from it, which its port bounds, in this kind as in bf16 and fp8.  The epilogue's pass through shared memory costs
+// 15 % of a K of 4096 alone and nothing under the cap; halves of 128 columns on three accumulators hid it no better.
 #include <cuda.h>
 
 #include <atomic>
@@ -29,7 +34,7 @@ namespace {
 namespace mx {
 
 constexpr int BM = 256, HALF_M = 128, BN = 256, HALF_N = 128, BK = 256;      // BK in elements: 128 bytes per row
-constexpr int STAGES = 5;
+constexpr int STAGES = 5;                                                    // 3 / 4 / 5 stages: 133 / 117 / 113 us at 8192 x 8192 x 4096
 constexpr int A_BYTES = HALF_M * BK / 2, B_BYTES = HALF_N * BK / 2;          // 16 KiB each
 constexpr int SF_TILE = 512;                                                 // scales of 128 rows x 128 elements
 constexpr int SFA_BYTES = 2 * SF_TILE, SFB_BYTES = 4 * SF_TILE;
@@ -559,16 +564,18 @@ int gemm_mxfp4(const void* A, const void* sa, const void* B, const void* sb, voi
   p.tma_epi = tma_epi;
   // Stages that a CTA goes through one after the other: `pair` in the pair kernel, `few` in the skinny one, whose stages take as
   // long for a quarter of the outputs, and whose sums pass through shared memory.  It is taken where it halves the stages of a call
-  // with at most 256 tokens, or does not lengthen them with at most 64.  us of the pair / skinny kernel, tokens x N x K: 17 x 4096 x
-  // 4096 10.5 / 6.2, 128: 10.8 / 8.1, 256: 11.1 / 10.4, 512: 11.3 / 12.6; 64 x 14336 x 4096 13.2 / 11.7; 300 x 14336 x 4096
-  // 18.7 / 30.1; 1024 x 1024 x 1024 7.4 / 8.5.
+  // with at most 256 tokens, or, with at most 64, where it shortens them or is one wave.  us of the pair / skinny kernel, tokens x N
+  // x K: 17 x 4096 x 4096 10.5 / 6.2, 128: 10.8 / 8.1, 256: 11.1 / 10.4, 512: 11.3 / 12.6; 64 x 4096 x 256 6.5 / 6.1; 17 x 14336 x
+  // 4096 13.9 / 12.7, x 28672 22.0 / 22.3, x 131072 75 / 87; 128 x 14336 x 4096 13.4 / 14.1; 300 x 14336 x 4096 18.7 / 30.1;
+  // 1024 x 1024 x 1024 7.4 / 8.5.
   const int clusters = num_sms / 2;
   const long long ctas = (N + skinny::TM - 1) / skinny::TM * ((M + skinny::TN - 1) / skinny::TN);
   int splits = 1;
   while (splits < 8 && ctas * splits * 2 <= num_sms && splits * 2 <= k_blocks) splits *= 2;
   const long long pair = (tiles + clusters - 1) / clusters * k_blocks;
   const long long few = (ctas * splits + num_sms - 1) / num_sms * ((k_blocks + splits - 1) / splits);
-  if (M <= 64 ? few <= pair : M <= 256 && 2 * few <= pair) {
+  const bool one_wave = ctas * splits <= num_sms;
+  if (M <= 64 ? few < pair || (few == pair && one_wave) : M <= 256 && 2 * few <= pair) {
     static std::atomic<bool> ready[4][64];
     const int which = splits == 1 ? 0 : splits == 2 ? 1 : splits == 4 ? 2 : 3;
     auto kernel = which == 0 ? skinny::gemm_mxfp4_skinny_kernel<1> : which == 1 ? skinny::gemm_mxfp4_skinny_kernel<2>
