@@ -193,6 +193,20 @@ def test_product(dev, out, M, N, K):
 
 
 @pytest.mark.parametrize("dev", LANES)
+@pytest.mark.parametrize("M,N,K", [(1, 18944, 96), (17, 18945, 288), (64, 20001, 32), (65, 19001, 64), (5, 37889, 544)])
+def test_product_few_tokens_of_a_wide_matrix(dev, M, N, K):
+    """Either side of one wave of 128-row tiles, where the choice between the two product kernels turns."""
+    k = lane(dev)
+    a, b = k.quant_mxfp4(rnd(dev, M, K, seed=M)), k.quant_mxfp4(rnd(dev, N, K, seed=N, scale=K ** -0.5))
+    A, B = unpack(k, *a).double(), unpack(k, *b).double()
+    for out in (BF, F32):
+        y = k.linear_mxfp4(*a, *b, out_dtype=out)
+        assert ((y.double() - A @ B.t()).abs() <= product_bound(A, B, K, out)).all()
+    if dev == "cuda":
+        assert native().gemm_mxfp4_last_error() == 0
+
+
+@pytest.mark.parametrize("dev", LANES)
 def test_product_reads_every_scale_where_it_belongs(dev):
     """One row and one block at a time carries a scale of its own; exact in fp32."""
     k = lane(dev)
