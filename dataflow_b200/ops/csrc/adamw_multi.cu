@@ -51,12 +51,13 @@ DFB_DEVICE uint32_t mix32(uint32_t x) {
 }
 
 // Square roots, rounded to nearest: Heron's step on an approximate reciprocal root with the residual from a fused product
-// (Markstein 1990, "Computation of elementary functions on the IBM RISC System/6000 processor"), checked against sqrtf over
-// whole binades: the same from 2^-90 up, a last place off now and then below 2^-102, 0 for 0).
+// (Markstein 1990, "Computation of elementary functions on the IBM RISC System/6000 processor").  For 2^-90 <= x < infinity, where
+// the residual x - s^2 is exact (its last bit is worth x 2^-48 or more).  Below, down to the smallest normal number, a last place may be
+// off, but the result is below 2^-45; of zero, a subnormal number, infinity and NaN the result is NaN.
 DFB_DEVICE float2 root2(float2 x) {
   float2 y;
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(fmaxf(x.x, 0x1p-126f)));
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(fmaxf(x.y, 0x1p-126f)));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(x.x));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(x.y));
   const float2 s = mul2(x, y);
   const float2 e = fma2(make_float2(-s.x, -s.y), s, x);
   return fma2(e, mul2(y, both(0.5f)), s);
@@ -177,14 +178,28 @@ DFB_DEVICE void step(const AdamTensor& t, const AdamHyper& h, Loaded<WK, GB, BIT
   const float2 one = both(h.one);
   const float2 b1 = both(h.b1), c1 = both(h.c1), b2 = both(h.b2), c2 = both(h.c2), gs = both(h.gscale);
   if constexpr (BITS8) {
-    float am = 0.f, ar = 0.f;
+    float am = 0.f, ar = 0.f, least = INFINITY;
+    auto square = [&](float2 g, int j) {
+      const float2 r0 = mul2(pair(in.v, j), both(in.sv));
+      return fma2(mul2(mul2(r0, r0), b2), one, mul2(mul2(g, g), c2));
+    };
 #pragma unroll
     for (int j = 0; j < P; ++j) {
-      const float2 g = mul2(pair(in.g, j), gs), r0 = mul2(pair(in.v, j), both(in.sv));
+      const float2 g = mul2(pair(in.g, j), gs);
       m[j] = fma2(mul2(mul2(pair(in.m, j), both(in.sm)), b1), one, mul2(g, c1));
-      r[j] = root2(fma2(mul2(mul2(r0, r0), b2), one, mul2(mul2(g, g), c2)));
+      r[j] = root2(square(g, j));
       am = fmaxf(am, fmaxf(fabsf(m[j].x), fabsf(m[j].y)));
       ar = fmaxf(ar, fmaxf(r[j].x, r[j].y));
+      least = min_nan(least, r[j].x, r[j].y);
+    }
+    if (!(least >= 0x1p-45f) && (HOW != kElements || i < n)) {      // some square is none that root2 takes: this thread's roots again
+      ar = 0.f;
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        const float2 x = square(mul2(pair(in.g, j), gs), j);
+        r[j] = make_float2(sqrtf(x.x), sqrtf(x.y));
+        ar = fmaxf(ar, fmaxf(r[j].x, r[j].y));
+      }
     }
     const float sm = fmaxf(__fmul_rn(max_lanes<128 / E>(am), 1.f / kE4M3Top), kMinScale);
     const float sr = fmaxf(__fmul_rn(max_lanes<128 / E>(ar), 1.f / kE4M3Top), kMinScale);
@@ -199,7 +214,7 @@ DFB_DEVICE void step(const AdamTensor& t, const AdamHyper& h, Loaded<WK, GB, BIT
     for (int j = 0; j < P; ++j) {
       y[j] = mul2(m[j], im);
       z[j] = mul2(r[j], ir);
-      low = min_nan(min_nan(low, min_nan(fabsf(y[j].x), fabsf(y[j].y))), min_nan(z[j].x, z[j].y));
+      low = min_nan(min_nan(low, fabsf(y[j].x), fabsf(y[j].y)), z[j].x, z[j].y);
     }
     uint32_t x = static_cast<uint32_t>(i) * 0x9e3779b9u + h.seed * 0x85ebca6bu + static_cast<uint32_t>(i >> 32) * 0xc2b2ae35u;
     // every value of the warp a normal code: almost always, where no moment is zero

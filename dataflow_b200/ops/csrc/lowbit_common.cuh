@@ -24,9 +24,9 @@ DFB_DEVICE float2 fma2(float2 a, float2 b, float2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(as_u64(a)), "l"(as_u64(b)), "l"(as_u64(c)));
   return as_f2(r);
 }
-DFB_DEVICE float min_nan(float a, float b) {      // the smaller one, or NaN if either is
+DFB_DEVICE float min_nan(float a, float b, float c) {      // the smallest one, or NaN if any is
   float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 

@@ -274,7 +274,8 @@ def adamw_multi_step(ws, gs, ms, vs, lr, beta1=0.9, beta2=0.95, eps=1e-8, wds=0.
         if bits8:
             r = _state_load(v, v_scales[i].view(-1))
             m1 = _state_load(m, m_scales[i].view(-1)) * beta1 + gf * (1 - beta1)
-            r1 = torch.sqrt((r * r) * beta2 + (gf * gf) * (1 - beta2))
+            # correctly rounded everywhere: torch's own 32-bit root on the CPU is a last place off now and then
+            r1 = torch.sqrt(((r * r) * beta2 + (gf * gf) * (1 - beta2)).double()).float()
             lo16, hi16 = state_dither(k, seed, w.device)
             _state_store(m1, m, m_scales[i].view(-1), lo16, 0.0)
             _state_store(r1, v, v_scales[i].view(-1), hi16, 2.0 ** -9)

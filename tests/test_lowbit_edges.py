@@ -1,0 +1,85 @@
+"""Narrow-format operators (``K.lowbit``) where their ranges end: squares below and above the normal numbers, rows whose statistic is
+not a number, lists and matrices long enough that a block walks on.  Runs on the plain-torch lane (CPU) and, on a device, on the kernels."""
+import math
+
+import pytest
+import torch
+
+from dataflow_b200.ops import lowbit_eager as E
+from dataflow_b200.ops import resolve_kernels
+
+BF, F32, F64, F8, U8 = torch.bfloat16, torch.float32, torch.float64, torch.float8_e4m3fn, torch.uint8
+LANES = [pytest.param("cpu", id="eager"), pytest.param("cuda", id="sm100", marks=pytest.mark.gpu)]
+
+
+def lane(dev):
+    return resolve_kernels(kernel_set="eager" if dev == "cpu" else None).lowbit
+
+
+def plain():
+    return resolve_kernels(kernel_set="eager").lowbit
+
+
+def same_bytes(a, b):
+    return torch.equal(a.contiguous().view(U8), b.contiguous().view(U8))
+
+
+# ------------------------------------------------------------------ AdamW: the root of the second moment
+def lone_gradients(n, seed):
+    """One gradient per block of 128, over the whole range of fp32, so that a block's scale tells its root."""
+    g = torch.Generator().manual_seed(seed)
+    e = torch.randint(-78, 64, (n,), generator=g)
+    v = torch.ldexp(1 + torch.rand(n, generator=g), e) * torch.where(torch.rand(n, generator=g) < 0.5, -1.0, 1.0)
+    ends = torch.tensor([0.0, -0.0, 1e-20, -3e-21, 1e-22, 4e-23, 1e-30, 1e-44, 1.9e19, 3e19, -1e20, 1e30, -1e38, 2.0 ** -63, 2.0 ** -45,
+                         2.0 ** -44, float("inf"), float("nan")])
+    v[:len(ends)] = ends
+    return v
+
+
+@pytest.mark.parametrize("dev", LANES)
+def test_adamw_8bit_root_over_the_whole_range(dev):
+    """The scale of a block with one gradient is the root of its square, both rounded as the definition says (a root in 64 bits,
+    rounded once to 32, is the correctly rounded one), from the smallest subnormal square up to squares that overflow."""
+    k, n = lane(dev), 1 << (13 if dev == "cpu" else 19)
+    lone = lone_gradients(n, 3)
+    x = (lone * lone) * torch.tensor(1 - 0.95, dtype=F32)
+    r = torch.sqrt(x.double()).float()
+    want = torch.where(r == r, r * torch.tensor(1 / 448, dtype=F32), torch.zeros(())).clamp(min=2.0 ** -120)
+    grad = torch.zeros(n, 128)
+    grad[:, 77] = lone
+    grad = grad.view(-1).to(dev)
+    w0 = torch.ones(n * 128, device=dev)
+    w, m, v = w0.clone(), torch.zeros(n * 128, device=dev).to(F8), torch.zeros(n * 128, device=dev).to(F8)
+    ms, vs = torch.zeros(n, device=dev), torch.zeros(n, device=dev)
+    k.adamw_multi_step([w], [grad], [m], [v], 1e-3, 0.9, 0.95, 1e-8, 0.0, 1, m_scales=[ms], v_scales=[vs])
+    bad = vs.cpu().view(torch.int32) != want.view(torch.int32)
+    assert not bad.any(), [(float(lone[i]), float(vs[i]), float(want[i])) for i in torch.nonzero(bad).view(-1)[:5].tolist()]
+    got = v.view(n, 128)[:, 77].float().cpu() * vs.cpu()
+    fine = r.isfinite()
+    # a block's largest code is 448 or, rounded down, 416
+    assert ((got - r).abs()[fine] <= r[fine] / 14 * (1 + 1e-6) + 2.0 ** -126).all() and torch.isnan(got[~fine]).all()
+    # a square that overflows is an infinite root: the weight stays; only an infinite gradient or a NaN takes it along
+    w = w.view(n, 128)[:, 77].cpu()
+    assert torch.equal(torch.isnan(w), ~lone.isfinite()) and (w[r == math.inf][lone[r == math.inf].isfinite()] == 1).all()
+
+
+@pytest.mark.gpu
+def test_adamw_lanes_agree_to_the_bit_over_the_whole_range():
+    """Whole blocks of tiny, ordinary and huge gradients, and states that these left behind, over three steps."""
+    g = torch.Generator().manual_seed(8)
+    n = 4096 * 128
+    size = torch.pow(10.0, torch.rand(n // 128, 1, generator=g, dtype=F64) * 44 - 24.5)
+    runs = []
+    grads = [(torch.randn(n // 128, 128, generator=g) * size).float().view(-1).cuda() for _ in range(2)] + [torch.zeros(n, device="cuda")]
+    for K in (lane("cuda"), plain()):
+        w, m, v = torch.ones(n, device="cuda"), torch.zeros(n, device="cuda").to(F8), torch.zeros(n, device="cuda").to(F8)
+        ms, vs = torch.zeros(n // 128, device="cuda"), torch.zeros(n // 128, device="cuda")
+        steps = []
+        for i, grad in enumerate(grads):
+            K.adamw_multi_step([w], [grad], [m], [v], 1e-3, step=i + 1, m_scales=[ms], v_scales=[vs])
+            steps.append([t.clone() for t in (m.float(), v.float(), ms, vs, w.isfinite().float())])
+        runs.append(steps)
+    for a, b in zip(*runs):
+        for i, (s, t) in enumerate(zip(a, b)):
+            assert torch.equal(torch.isnan(s), torch.isnan(t)), i
+            assert torch.equal(torch.nan_to_num(s, nan=-1.0), torch.nan_to_num(t, nan=-1.0)), i
