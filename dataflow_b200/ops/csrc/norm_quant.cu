@@ -83,8 +83,9 @@ DFB_DEVICE void emit(const float* f, float inv, bool on, uint8_t* q, uint8_t* ti
     constexpr int kLanes = kMxBlock / E;
     float amax = mx_amax8(f);
     if constexpr (E == 16) amax = max_nan(amax, mx_amax8(f + 8));
-    const uint32_t sb = mx_scale_byte(mx_amax_lanes<kLanes>(amax));
-    const uint32_t word = mx_scale_word<kLanes>(sb);          // columns that do not exist count as zero blocks
+    amax = mx_amax_lanes<kLanes>(amax);
+    const uint32_t sb = on ? mx_scale_byte(amax) : 0u;        // a block lies inside the row or behind it; there y is NaN where rstd is
+    const uint32_t word = mx_scale_word<kLanes>(sb);
     if (on) {
       const float x = mx_scale_inv(sb);
       if constexpr (E == 16) *reinterpret_cast<uint2*>(q + v * 8) = make_uint2(mx_scale_pack8(f, x), mx_scale_pack8(f + 8, x));

@@ -83,3 +83,31 @@ def test_adamw_lanes_agree_to_the_bit_over_the_whole_range():
         for i, (s, t) in enumerate(zip(a, b)):
             assert torch.equal(torch.isnan(s), torch.isnan(t)), i
             assert torch.equal(torch.nan_to_num(s, nan=-1.0), torch.nan_to_num(t, nan=-1.0)), i
+
+
+# ------------------------------------------------------------------ the norm: rows whose statistic is not a number
+@pytest.mark.parametrize("dev", LANES)
+@pytest.mark.parametrize("cols", [32, 96, 352, 608, 1056, 2080, 4128, 8224, 16416])
+@pytest.mark.parametrize("off", [0, 8], ids=["on32", "on16"])
+def test_norm_scale_bytes_past_the_blocks_are_zero_in_every_row(dev, cols, off):
+    """A NaN, an infinity and statistics that are neither: the row's own blocks may be NaN, the bytes behind them are zero, and the
+    other rows are those of a call without these."""
+    k, g = lane(dev), torch.Generator().manual_seed(cols)
+    buf = torch.randn(6, cols + 32, generator=g).to(BF).to(dev)
+    w = torch.randn(cols, generator=g).to(BF).to(dev)
+    clean = k.rmsnorm_mxfp4(buf[:, off:off + cols], w)
+    bad = buf.clone()
+    bad[1, off + cols - 1], bad[4, off] = float("nan"), float("inf")
+    for res in (None, torch.zeros_like(buf)[:, off:off + cols]):
+        q, s, _, rstd = k.rmsnorm_mxfp4(bad[:, off:off + cols], w, residual=res)
+        assert torch.isnan(rstd[1]) and rstd[4] == 0
+        rows = E.mxfp4_scale_rows(s, 6, cols)
+        assert torch.equal(E.mxfp4_scale_tiles(rows), s)
+        assert (rows[1] == 255).all()
+        for r in (0, 2, 3, 5):
+            assert torch.equal(q[r], clean[0][r]) and torch.equal(rows[r], E.mxfp4_scale_rows(clean[1], 6, cols)[r])
+    for value in (float("nan"), float("inf"), -float("inf")):
+        given = clean[3].clone()
+        given[3] = value
+        s = k.rmsnorm_mxfp4(buf[:, off:off + cols], w, rstd=given)[1]
+        assert torch.equal(E.mxfp4_scale_tiles(E.mxfp4_scale_rows(s, 6, cols)), s)
