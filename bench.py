@@ -183,7 +183,7 @@ def bench_ours(a) -> dict:
     out = {
         "metric": "train_tokens_per_s", "value": value, "unit": "tokens/s", "n_gpus": world, "steps": a.steps,
         "warmup": a.warmup, "ms_per_step": dev_s / a.steps * 1e3, "higher_is_better": True, "scaling": "weak",
-        "vs_baseline": value / BASELINE_TOK_S, "dtype": "bf16" if a.linear_precision == "bf16" else f"bf16 ({a.linear_precision} forward projections)",
+        "vs_baseline": value / BASELINE_TOK_S, "dtype": "bf16" if tr.linear_precision == "bf16" else f"bf16 ({tr.linear_precision} forward projections)",
         "data": "synthetic", "impl": "ours",
         "config": {"model": a.preset + (f"-cut{a.layers}L" if a.layers else ""), "global_batch": tokens_step * world // a.seq_len,
                    "seq_len": a.seq_len, "tokens_per_step": tokens_step * world,

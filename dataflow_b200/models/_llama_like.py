@@ -5,7 +5,7 @@ from __future__ import annotations
 
 import dataclasses
 
-from .families import ModelFamily, register_family
+from .families import LINEAR_PRECISIONS, ModelFamily, register_family
 from .llama3.blocks import build_llama3_resolver
 from .llama3.model import (ShapedLlama3Config, derive_dims, family_layouts, flops_per_token, initial_values, lower_llama3)
 
@@ -28,4 +28,4 @@ def register_llama_like(name: str, presets: dict, **fixed):
         initial_values=initial_values, build_resolver=build_llama3_resolver,
         family_layouts=lambda dims, policy=None, optimizer="adamw": family_layouts(dims, policy, optimizer),
         presets={k: make(v) for k, v in presets.items()}, twin=_twin, bridge=_bridge, block_kinds=("block",),
-        flops_per_token=flops_per_token))
+        flops_per_token=flops_per_token, linear_precisions=LINEAR_PRECISIONS))

@@ -546,4 +546,5 @@ def register_torch_family(spec: TorchFamilySpec) -> ModelFamily:
         build_resolver=lambda dims, hyper, kernels, device, layouts=None, policy=None: build_resolver(spec, dims, hyper, kernels, device, layouts, policy),
         family_layouts=lambda dims, policy=None, optimizer="adamw": layouts(spec, dims, policy, optimizer),
         presets=dict(spec.presets), twin=lambda cfg: make_twin(spec, cfg), bridge=lambda cfg, views_of: bridge(spec, cfg, views_of),
-        block_kinds=tuple(dict.fromkeys(k for p in spec.presets.values() for k in spec.layer_kinds(p()))), flops_per_token=None))
+        block_kinds=tuple(dict.fromkeys(k for p in spec.presets.values() for k in spec.layer_kinds(p()))), flops_per_token=None,
+        linear_precisions=("bf16",)))        # in the forms: a configuration with the field chooses there

@@ -6,6 +6,7 @@ environment variable (comma-separated module names).  Contract parity: reference
 """
 from __future__ import annotations
 
+import dataclasses
 import importlib
 import os
 from dataclasses import dataclass, field
@@ -28,6 +29,37 @@ class ModelFamily:
     bridge: Callable[..., Mapping[str, Any]] | None = None   # engine views -> twin state_dict
     block_kinds: tuple[str, ...] = ()
     flops_per_token: Callable[[Any], float] | None = None
+    # operand precisions of the dense forward projections that the family's blocks take from ``hyper["linear_precision"]``; a family
+    # whose configuration has a ``linear_precision`` field gets it there instead.  None: not stated (a plugin's own matter)
+    linear_precisions: tuple[str, ...] | None = None
+
+
+LINEAR_PRECISIONS = ("bf16", "fp8", "mxfp4")
+
+
+class LinearPrecisionError(ValueError):
+    """A run asks for projections in a precision that does not exist or that its family's blocks do not compute."""
+
+
+def check_linear_precision(value) -> str:
+    if value not in LINEAR_PRECISIONS:
+        raise LinearPrecisionError(f"linear_precision must be bf16, fp8 or mxfp4, not {value!r}")
+    return value
+
+
+def with_linear_precision(fam: ModelFamily, cfg, hyper: Mapping[str, Any] | None):
+    """``cfg`` as the run uses it: the precision that the hyper-parameters name, carried into the configurations that hold it and
+    refused for families that would not compute it.  Hyper-parameters that name none leave the configuration's own."""
+    p = (hyper or {}).get("linear_precision")
+    if p is None:
+        return cfg
+    check_linear_precision(p)
+    if "linear_precision" in {f.name for f in dataclasses.fields(cfg)}:
+        return cfg if cfg.linear_precision == p else dataclasses.replace(cfg, linear_precision=p)
+    if fam.linear_precisions is not None and p not in fam.linear_precisions:
+        raise LinearPrecisionError(f"linear_precision {p!r}: the blocks of family {fam.name!r} compute their projections in "
+                                   f"{' / '.join(fam.linear_precisions)} only")
+    return cfg
 
 
 _FAMILIES: dict[str, ModelFamily] = {}

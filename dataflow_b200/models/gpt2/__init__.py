@@ -37,4 +37,5 @@ FAMILY = register_family(ModelFamily(
     name="gpt2", config_type=ShapedGpt2Config, derive_dims=derive_dims, lower=lower_gpt2,
     initial_values=initial_values, build_resolver=build_gpt2_resolver,
     family_layouts=lambda dims, policy=None, optimizer="adamw": family_layouts(dims, policy, optimizer),
-    presets=PRESETS, twin=_twin, bridge=_bridge, block_kinds=("block",), flops_per_token=flops_per_token))
+    presets=PRESETS, twin=_twin, bridge=_bridge, block_kinds=("block",), flops_per_token=flops_per_token,
+    linear_precisions=("bf16",)))

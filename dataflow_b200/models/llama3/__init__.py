@@ -1,7 +1,7 @@
 """llama3 family registration and presets (tiny, the l3 ladder, 8B, 70B)."""
 from __future__ import annotations
 
-from ..families import ModelFamily, register_family
+from ..families import LINEAR_PRECISIONS, ModelFamily, register_family
 from .blocks import build_llama3_resolver
 from .model import (Llama3Dims, ShapedLlama3Config, derive_dims, family_layouts, flops_per_token,
                     initial_values, lower_llama3)
@@ -46,4 +46,5 @@ def _bridge(cfg, views_of):
 FAMILY = register_family(ModelFamily(
     name="llama3", config_type=ShapedLlama3Config, derive_dims=derive_dims, lower=lower_llama3,
     initial_values=initial_values, build_resolver=build_llama3_resolver, family_layouts=_layouts,
-    presets=PRESETS, twin=_twin, bridge=_bridge, block_kinds=("block",), flops_per_token=flops_per_token))
+    presets=PRESETS, twin=_twin, bridge=_bridge, block_kinds=("block",), flops_per_token=flops_per_token,
+    linear_precisions=LINEAR_PRECISIONS))

@@ -134,4 +134,5 @@ FAMILY = register_family(ModelFamily(
     build_resolver=build_tp_resolver,
     family_layouts=lambda dims, policy=None, optimizer="adamw": family_layouts(dims, policy, optimizer),
     presets={k: (lambda kw=v: ShapedLlama3Config(**{**kw, "family": "tp_mlp"})) for k, v in PRESETS.items()},
-    twin=None, bridge=None, block_kinds=("block",), flops_per_token=flops_per_token))
+    twin=None, bridge=None, block_kinds=("block",), flops_per_token=flops_per_token,
+    linear_precisions=("bf16",)))

@@ -33,11 +33,11 @@ class FamilyInitExecutable:
 
 
 def build_model_family_resolver(spec: Mapping[str, Any], env):
-    from .models.families import resolve_family
+    from .models.families import resolve_family, with_linear_precision
     from .ops import resolve_kernels
     from .run.presets import cfg_from_dict
     fam = resolve_family(spec["family"])
-    cfg = cfg_from_dict(fam, spec["cfg"])
+    cfg = with_linear_precision(fam, cfg_from_dict(fam, spec["cfg"]), spec.get("hyper"))
     device = getattr(env, "device", None)
     kernel_set = getattr(env, "kernel_set", None)
     K = resolve_kernels(kernel_set=("eager" if device is None and kernel_set is None else kernel_set))

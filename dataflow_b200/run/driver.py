@@ -20,7 +20,7 @@ from typing import Any, Mapping
 from ..core import Program
 from ..lowering.planning import PlannedProgram, plan_program
 from ..lowering.shaped_program import ShapedHardware, resolve_hardware
-from ..models.families import resolve_family
+from ..models.families import resolve_family, with_linear_precision
 from ..runtime import Buffer, CpuBackend, Engine, Session
 
 GiB = 1 << 30
@@ -126,7 +126,9 @@ class Trainer:
         import torch
         from ..ops import resolve_kernels
         self.fam = resolve_family(family)
-        self.cfg = cfg
+        self.cfg = cfg = with_linear_precision(self.fam, cfg, hyper)
+        # operand precision of the dense forward projections
+        self.linear_precision = getattr(cfg, "linear_precision", None) or (hyper or {}).get("linear_precision") or "bf16"
         self.device = device
         self.verbose = verbose
         self.hyper = {"optimizer": getattr(cfg, "optimizer", "adamw"),

@@ -165,8 +165,9 @@ def reference_loop(family: str, cfg, factory: Callable, steps: int, hyper: Mappi
     """The pure-torch twin on the same packed data (fp32 autograd + torch.optim.AdamW): the oracle curve."""
     import torch
     from ..blocks.optim import lr_at
-    from ..models.families import resolve_family
+    from ..models.families import resolve_family, with_linear_precision
     fam = resolve_family(family)
+    cfg = with_linear_precision(fam, cfg, hyper)
     twin = fam.twin(cfg)
     if views_of is not None:
         twin.load_state_dict(fam.bridge(cfg, views_of))

@@ -9,6 +9,7 @@ from dataclasses import asdict, dataclass
 from typing import Any
 
 from ..blocks.optim import LRSchedule
+from ..models.families import check_linear_precision
 
 
 @dataclass(frozen=True)
@@ -26,11 +27,13 @@ class Recipe:
     optimizer: str = "adamw"
     muon_lr: float | None = None
     momentum: float = 0.95
-    linear_precision: str = "bf16"      # bf16 | fp8 | mxfp4: operand precision of the dense forward projections (llama-like families)
+    # bf16 | fp8 | mxfp4: operand precision of the dense forward projections; None: the configuration's own.  A family whose blocks
+    # do not compute it refuses the run
+    linear_precision: str | None = None
 
     def __post_init__(self):
-        if self.linear_precision not in ("bf16", "fp8", "mxfp4"):
-            raise ValueError(f"linear_precision must be bf16, fp8 or mxfp4, not {self.linear_precision!r}")
+        if self.linear_precision is not None:
+            check_linear_precision(self.linear_precision)
 
     def lr_schedule(self) -> LRSchedule:
         return LRSchedule(self.schedule, self.peak_lr, self.min_lr, self.warmup_steps, self.total_steps, self.decay_steps)
@@ -43,7 +46,7 @@ class Recipe:
              "beta2": self.beta2, "eps": self.eps, "weight_decay": self.weight_decay, "momentum": self.momentum}
         if self.muon_lr is not None:
             h["muon_lr"] = self.muon_lr
-        if self.linear_precision != "bf16":
+        if self.linear_precision is not None:
             h["linear_precision"] = self.linear_precision
         return h
 

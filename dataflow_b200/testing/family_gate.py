@@ -41,7 +41,7 @@ def run_pair(family: str, *, device: int | None = None, policy: str = "fp32", st
                     for v in tr.views_of(oid, tr.layouts.layout_of(oid)).values():
                         if v.dim() >= 2:
                             v.mul_(hot_mult)
-        twin = fam.twin(cfg)
+        twin = fam.twin(tr.cfg)
         twin.load_state_dict(fam.bridge(cfg, tr.views_of))
         import fnmatch
         only = tuple(getattr(cfg, "trainable_patterns", ()) or ())          # runs that update a named subset of fields

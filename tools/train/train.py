@@ -266,11 +266,13 @@ def main(argv=None) -> int:
            "scaling": cmd_scaling, "peek": cmd_peek, "compare": cmd_compare}[a.cmd]
     if os.environ.get("DATAFLOW_TRACEBACK") == "1":
         return run(a, argv)
+    from dataflow_b200.models.families import LinearPrecisionError
     from dataflow_b200.sim.policies.pressurefit import PlanningError
     try:
         return run(a, argv)
-    except (KeyError, FileNotFoundError, PlanningError) as e:
-        # a name that does not exist (preset, optimizer, data scheme, checkpoint) or a budget nothing fits: the user's to fix,
+    except (KeyError, FileNotFoundError, PlanningError, LinearPrecisionError) as e:
+        # a name that does not exist (preset, optimizer, data scheme, checkpoint), a precision the family does not compute or a budget
+        # nothing fits: the user's to fix,
         # one line instead of a traceback (DATAFLOW_TRACEBACK=1 shows where it was raised)
         msg = e.args[0] if isinstance(e, KeyError) and e.args else str(e)
         print(f"train.py {a.cmd}: {msg}", file=sys.stderr)
