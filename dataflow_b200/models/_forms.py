@@ -9,6 +9,8 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 
+from .families import check_linear_precision
+
 
 def rmsnorm(x, w, eps: float):
     xf = x.float()
@@ -88,6 +90,7 @@ class _LinearMxfp4(torch.autograd.Function):
 def linear(x, w, precision: str = "bf16"):
     """x (n, k) @ w (k, m); ``precision="fp8"``: e4m3 operands in the forward (see ``ops`` ``linear_fwd_fp8``); ``"mxfp4"``:
     4-bit operands.  A contraction length the format does not take (fp8: 16s, mxfp4: 32s) falls back to the plain product."""
+    check_linear_precision(precision)
     if precision == "mxfp4" and x.dim() == 2 and x.shape[1] % 32 == 0:
         return _LinearMxfp4.apply(x, w)
     if precision == "fp8" and x.dim() == 2 and x.shape[1] % 16 == 0 and w.shape[1] % 16 == 0:

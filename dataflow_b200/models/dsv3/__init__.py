@@ -12,6 +12,7 @@ from typing import Any
 from ...blocks.layouts import DTypePolicy, Field
 from .. import _forms as F
 from .._torch_family import TorchFamilySpec, register_torch_family
+from ..families import check_linear_precision
 
 
 @dataclass(frozen=True)
@@ -60,8 +61,12 @@ class Dsv3Config:
     ep: int = 1
     ep_capacity: float = 2.0
     # "fp8": the dense and shared-expert MLP projections and the attention output projection run their forward on e4m3
-    # operands (per-row / per-column scales); the routed experts' grouped GEMMs and every backward product stay bf16
+    # operands (per-row / per-column scales), "mxfp4": on 4-bit operands; the routed experts' grouped GEMMs and every backward
+    # product stay bf16
     linear_precision: str = "bf16"
+
+    def __post_init__(self):
+        check_linear_precision(self.linear_precision)
 
     @property
     def trainable_patterns(self) -> tuple[str, ...]:

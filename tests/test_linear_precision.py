@@ -96,3 +96,20 @@ def test_the_command_line_refuses_in_one_line():
     r = subprocess.run([sys.executable, "tools/train/train.py", "train", "--preset", "gpt2:tiny", "--device", "cpu", "--steps", "1",
                         "--linear-precision", "mxfp4"], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert r.returncode == 2 and "linear_precision" in r.stderr and "Traceback" not in r.stderr, r.stderr
+
+
+def test_an_unknown_precision_is_refused_where_it_is_written():
+    """In the configuration and in the form itself: a value that no branch knows used to run as the plain product."""
+    import torch
+    from dataflow_b200.models import _forms as F
+    for family in ("dsv3", "dsv32", "glm52"):
+        cfg = resolve_family(family).presets["tiny"]()
+        for p in ("fp4", "mxfp8", "", None):
+            with pytest.raises(ValueError, match="linear_precision"):
+                dataclasses.replace(cfg, linear_precision=p)
+    x, w = torch.zeros(3, 64), torch.zeros(64, 5)
+    for p in ("fp4", "", None):
+        with pytest.raises(ValueError, match="linear_precision"):
+            F.linear(x, w, p)
+        with pytest.raises(ValueError, match="linear_precision"):
+            F.swiglu_mlp(x, torch.zeros(64, 64), torch.zeros(32, 5), p)
