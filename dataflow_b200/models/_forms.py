@@ -63,13 +63,22 @@ class _LinearFp8(torch.autograd.Function):
         return dy @ w.t(), x.t() @ dy
 
 
+def _gemm_operand(t):
+    """``t`` as the bf16 GEMMs take it: contiguous, and starting on 16 bytes (a view need not)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 class _LinearMxfp4(torch.autograd.Function):
     """y = x @ w with both operands rounded to the microscaled 4-bit format along the contraction in the forward (see ``ops``
-    ``lowbit.linear_fwd_mxfp4``); the backward passes the rounding straight through, on the unquantised operands."""
+    ``lowbit.linear_fwd_mxfp4``); the backward passes the rounding straight through, on the unquantised operands: by the native
+    bf16 GEMMs where these take the width (a multiple of 8), else by the plain products."""
 
     @staticmethod
     def forward(ctx, x, w):
         from ..ops import resolve_kernels
+        if x.dtype != w.dtype:
+            raise ValueError(f"linear: x and w have one type, not {x.dtype} and {w.dtype}")
         ks = _native(x) or resolve_kernels(kernel_set="eager")
         ctx.save_for_backward(x, w)
         return ks.lowbit.linear_fwd_mxfp4(x.contiguous(), w.contiguous())
@@ -82,7 +91,7 @@ class _LinearMxfp4(torch.autograd.Function):
         ks = _native(dy) if w.shape[1] % 8 == 0 and dy.shape[0] else None
         if ks is None:
             return dy @ w.t() if need_x else None, x.t() @ dy if need_w else None
-        x, w, dy = x.contiguous(), w.contiguous(), dy.contiguous()
+        x, w, dy = _gemm_operand(x), _gemm_operand(w), _gemm_operand(dy)
         dw = ks.linear_wgrad_bf16(x, dy, torch.empty_like(w)) if need_w else None
         return ks.linear_dgrad_bf16(dy, w) if need_x else None, dw
 

@@ -111,3 +111,33 @@ def test_norm_scale_bytes_past_the_blocks_are_zero_in_every_row(dev, cols, off):
         given[3] = value
         s = k.rmsnorm_mxfp4(buf[:, off:off + cols], w, rstd=given)[1]
         assert torch.equal(E.mxfp4_scale_tiles(E.mxfp4_scale_rows(s, 6, cols)), s)
+
+
+# ------------------------------------------------------------------ the linear form: what the forward takes, the backward takes
+@pytest.mark.parametrize("dev", LANES)
+@pytest.mark.parametrize("m", [32, 7], ids=["m32", "m7"])
+def test_linear_form_of_views_that_start_anywhere(dev, m):
+    """Contiguous views one element into their storage, and a gradient that is one: the same numbers as of copies on their own."""
+    from dataflow_b200.models import _forms as F
+    n, k = 48, 64
+    dt = BF if dev == "cuda" else F32
+    g = torch.Generator().manual_seed(4)
+    flat = [torch.randn(a * b + 1, generator=g).to(dt).to(dev) for a, b in ((n, k), (k, m), (n, m))]
+    off = [t[1:].view(a, b) for t, (a, b) in zip(flat, ((n, k), (k, m), (n, m)))]
+    on = [t.clone() for t in off]
+    assert all(t.is_contiguous() and t.data_ptr() % 16 for t in off)
+    outs = []
+    for x, w, dy in (on, off):
+        x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        y = F.linear(x, w, "mxfp4")
+        outs.append((y.detach(), *torch.autograd.grad(y, [x, w], dy)))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
+def test_linear_form_refuses_operands_of_two_types():
+    """The plain product does, and the backward would."""
+    from dataflow_b200.models import _forms as F
+    for a, b in ((BF, F32), (F32, BF)):
+        with pytest.raises(ValueError, match="one type"):
+            F.linear(torch.zeros(3, 64, dtype=a), torch.zeros(64, 8, dtype=b), "mxfp4")
