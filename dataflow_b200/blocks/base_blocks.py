@@ -12,8 +12,8 @@ number.  Contract parity: reference ``src/dataflow_training/blocks/base_blocks.p
 from __future__ import annotations
 
 import fnmatch
-
 import math
+import zlib
 from typing import Any, Mapping
 
 from ..data.segments import resolve_segments
@@ -247,7 +247,10 @@ class OptimizerStep(_Base):
             self.K.lowbit.adamw_multi_step([w_.reshape(-1) for _, w_, _, _ in fs], [g_.reshape(-1) for _, _, g_, _ in fs], slot("s0"),
                                            slot("s1"), lr, b1, b2, eps, [d for _, _, _, d in fs], step,
                                            masters=slot("master") if extra == "master" else None, los=slot("mlo") if extra == "mlo" else None,
-                                           m_scales=slot("s0_scale"), v_scales=slot("s1_scale"))
+                                           m_scales=slot("s0_scale"), v_scales=slot("s1_scale"),
+                                           # random bits of its own for every field of every layer, the same in every run
+                                           seed=[(zlib.crc32(f"{ctx.inputs[0].object_id}.{name}".encode()) + step) & 0xFFFFFFFF
+                                                 for name, _, _, _ in fs])
 
 
 def common_executables(dims, layouts, kernels, device, hyper) -> dict[str, Any]:

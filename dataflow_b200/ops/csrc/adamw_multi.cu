@@ -216,7 +216,7 @@ DFB_DEVICE void step(const AdamTensor& t, const AdamHyper& h, Loaded<WK, GB, BIT
       z[j] = mul2(r[j], ir);
       low = min_nan(min_nan(low, fabsf(y[j].x), fabsf(y[j].y)), z[j].x, z[j].y);
     }
-    uint32_t x = static_cast<uint32_t>(i) * 0x9e3779b9u + h.seed * 0x85ebca6bu + static_cast<uint32_t>(i >> 32) * 0xc2b2ae35u;
+    uint32_t x = static_cast<uint32_t>(i) * 0x9e3779b9u + t.seed * 0x85ebca6bu + static_cast<uint32_t>(i >> 32) * 0xc2b2ae35u;
     // every value of the warp a normal code: almost always, where no moment is zero
     if (__all_sync(0xffffffffu, low == 0x1p-6f)) {
 #pragma unroll

@@ -198,7 +198,7 @@ void adamw_multi(const std::vector<Tensor>& ws, const std::vector<Tensor>& gs, c
                  double lr, double b1, double b2, double eps, const std::vector<double>& wds, int64_t step,
                  const c10::optional<std::vector<Tensor>>& masters, const c10::optional<std::vector<Tensor>>& los,
                  const c10::optional<std::vector<Tensor>>& m_scales, const c10::optional<std::vector<Tensor>>& v_scales, double gscale,
-                 int64_t seed) {
+                 int64_t seed, const c10::optional<std::vector<int64_t>>& seeds) {
   const char* op = "adamw_multi_step";
   const size_t n = ws.size();
   auto len = [&](const char* name, size_t k) { REFUSE_UNLESS(k == n, op, ": ", name, " has one entry per tensor"); };
@@ -207,6 +207,7 @@ void adamw_multi(const std::vector<Tensor>& ws, const std::vector<Tensor>& gs, c
   if (los.has_value()) len("los", los->size());
   if (m_scales.has_value()) len("m_scales", m_scales->size());
   if (v_scales.has_value()) len("v_scales", v_scales->size());
+  if (seeds.has_value()) len("seed", seeds->size());
   REFUSE_UNLESS(!(masters.has_value() && los.has_value()), op, ": masters and los exclude each other");
   REFUSE_UNLESS(step >= 1, op, ": step counts from 1");
   if (!n) return;
@@ -238,6 +239,7 @@ void adamw_multi(const std::vector<Tensor>& ws, const std::vector<Tensor>& gs, c
     dfb::AdamTensor t{};
     t.n = k;
     t.wd = (float)wds[i];
+    t.seed = static_cast<uint32_t>(seeds.has_value() ? (*seeds)[i] : seed);
     t.w = take(ws[i], wt, k, "weights are all bf16 or all fp32", true);
     t.g = take(gs[i], gt, k, "gradients are all bf16 or all fp32", false);
     t.m = take(ms[i], st, k, "moments are all fp32 or all float8_e4m3fn", true);
@@ -268,7 +270,6 @@ void adamw_multi(const std::vector<Tensor>& ws, const std::vector<Tensor>& gs, c
   h.inv_bc1 = (float)(1.0 / (1.0 - std::pow(b1, (double)step)));
   h.inv_sqrt_bc2 = (float)(1.0 / std::sqrt(1.0 - std::pow(b2, (double)step)));
   h.gscale = (float)gscale;
-  h.seed = static_cast<uint32_t>(seed);
   const int weights = masters.has_value() ? dfb::kAdamMaster : los.has_value() ? dfb::kAdamSplit : wt == at::kFloat ? dfb::kAdamF32 : dfb::kAdamBf16;
   launched(dfb::adamw_multi(table.data(), (int)table.size(), weights, gt == at::kFloat, bits8, h, sms(ws[0]), stream_of(ws[0])), op);
 }

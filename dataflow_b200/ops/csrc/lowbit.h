@@ -17,11 +17,11 @@ struct AdamTensor {
   float* v_scale;
   long long n;
   float wd;
+  uint32_t seed;          // of the 8-bit rounding
 };
 enum AdamWeights { kAdamBf16 = 0, kAdamF32 = 1, kAdamMaster = 2, kAdamSplit = 3 };
 struct AdamHyper {
   float lr, b1, c1, b2, c2, eps, inv_bc1, inv_sqrt_bc2, gscale;
-  uint32_t seed;
   float one = 1.f;
 };
 int adamw_multi(const AdamTensor* t, int count, int weights, bool g_f32, bool bits8, const AdamHyper& h, int num_sms, cudaStream_t s);

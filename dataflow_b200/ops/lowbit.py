@@ -59,6 +59,7 @@ def rmsnorm_mxfp4(x, w, eps: float = 1e-5, residual=None, rstd=None, h_out=None)
 def adamw_multi_step(ws, gs, ms, vs, lr, beta1=0.9, beta2=0.95, eps=1e-8, wds=0.0, step=1, masters=None, los=None,
                      m_scales=None, v_scales=None, gscale=1.0, seed=None):
     wds = [float(wds)] * len(ws) if isinstance(wds, (int, float)) else wds
+    each = isinstance(seed, (list, tuple))
     native().adamw_multi(ws, gs, ms, vs, lr, beta1, beta2, eps, wds, step, masters, los, m_scales, v_scales, gscale,
-                         (step if seed is None else seed) & 0xFFFFFFFF)
+                         0 if each else (step if seed is None else seed) & 0xFFFFFFFF, [s & 0xFFFFFFFF for s in seed] if each else None)
     return ws

@@ -231,8 +231,8 @@ def adamw_multi_step(ws, gs, ms, vs, lr, beta1=0.9, beta2=0.95, eps=1e-8, wds=0.
     ws bf16 (alone, or the working copy of an fp32 ``masters``, or the high half of a split master whose int16 low halves are
     ``los``) or fp32; gs bf16 or fp32; moments fp32, or 8 bits (``float8_e4m3fn``, with ``m_scales`` / ``v_scales`` fp32 of
     ceil(n / 128) entries; ``vs`` then holds the root of the second moment).  One choice of types per call.  ``wds``: weight
-    decay, a number or one per tensor.  ``seed`` of the 8-bit rounding defaults to ``step``.  The result of a tensor does not
-    depend on the others in the list."""
+    decay, a number or one per tensor.  ``seed`` of the 8-bit rounding, a number or one per tensor, defaults to ``step``: element
+    i of every tensor then rounds with the same random bits.  The result of a tensor does not depend on the others in the list."""
     n = len(ws)
     lists = [("gs", gs), ("ms", ms), ("vs", vs), ("masters", masters), ("los", los), ("m_scales", m_scales), ("v_scales", v_scales)]
     for name, l in lists:
@@ -249,7 +249,8 @@ def adamw_multi_step(ws, gs, ms, vs, lr, beta1=0.9, beta2=0.95, eps=1e-8, wds=0.
     for (_, end, a), (start, _, b) in zip(spans, spans[1:]):
         _need(start >= end or not (a or b), "adamw_multi_step: a tensor that is written appears twice or overlaps another")
     bc1, bc2 = 1 - beta1 ** int(step), 1 - beta2 ** int(step)
-    seed = int(step) if seed is None else int(seed)
+    seeds = list(seed) if isinstance(seed, (list, tuple)) else [int(step) if seed is None else int(seed)] * n
+    _need(len(seeds) == n, "adamw_multi_step: seed has one entry per tensor")
     for i in range(n):
         w, g, m, v = ws[i], gs[i], ms[i], vs[i]
         k = w.numel()
@@ -276,7 +277,7 @@ def adamw_multi_step(ws, gs, ms, vs, lr, beta1=0.9, beta2=0.95, eps=1e-8, wds=0.
             m1 = _state_load(m, m_scales[i].view(-1)) * beta1 + gf * (1 - beta1)
             # correctly rounded everywhere: torch's own 32-bit root on the CPU is a last place off now and then
             r1 = torch.sqrt(((r * r) * beta2 + (gf * gf) * (1 - beta2)).double()).float()
-            lo16, hi16 = state_dither(k, seed, w.device)
+            lo16, hi16 = state_dither(k, seeds[i], w.device)
             _state_store(m1, m, m_scales[i].view(-1), lo16, 0.0)
             _state_store(r1, v, v_scales[i].view(-1), hi16, 2.0 ** -9)
         else:

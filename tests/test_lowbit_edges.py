@@ -141,3 +141,62 @@ def test_linear_form_refuses_operands_of_two_types():
     for a, b in ((BF, F32), (F32, BF)):
         with pytest.raises(ValueError, match="one type"):
             F.linear(torch.zeros(3, 64, dtype=a), torch.zeros(64, 8, dtype=b), "mxfp4")
+
+
+# ------------------------------------------------------------------ AdamW: random bits of several tensors
+def eight_bit(dev, sizes, seed):
+    g = torch.Generator().manual_seed(seed)
+    mk = lambda n, s: torch.randn(n, generator=g).mul(s).to(dev)
+    zero = lambda n: torch.zeros(n, device=dev)
+    return {"ws": [mk(n, 0.05) for n in sizes], "gs": [mk(n, 1e-2) for n in sizes], "ms": [mk(n, 9).to(F8) for n in sizes],
+            "vs": [mk(n, 9).abs().to(F8) for n in sizes], "m_scales": [zero(-(-n // 128)) + 1e-4 for n in sizes],
+            "v_scales": [zero(-(-n // 128)) + 1e-4 for n in sizes]}
+
+
+def adam8(k, st, **kw):
+    k.adamw_multi_step(st["ws"], st["gs"], st["ms"], st["vs"], 1e-3, wds=0.1, step=3, m_scales=st["m_scales"], v_scales=st["v_scales"], **kw)
+
+
+@pytest.mark.parametrize("dev", LANES)
+def test_adamw_takes_a_seed_per_tensor(dev):
+    """A list of seeds is one call per tensor with its own; a number is the same for all, and the step where there is none."""
+    k, sizes, seeds = lane(dev), [300 + 40 * i for i in range(30)], [(7 * i * i + 1) * 0x12345 for i in range(30)]
+    runs = {}
+    for name, kw in (("list", {"seed": seeds}), ("number", {"seed": 3}), ("same", {"seed": [3] * 30}), ("none", {})):
+        adam8(k, runs.setdefault(name, eight_bit(dev, sizes, 1)), **kw)
+    one = eight_bit(dev, sizes, 1)
+    for i, s in enumerate(seeds):
+        adam8(k, {n: [t[i]] for n, t in one.items()}, seed=s)
+    for n in one:
+        for i in range(30):
+            assert same_bytes(runs["list"][n][i], one[n][i]) and same_bytes(runs["number"][n][i], runs["same"][n][i])
+            assert same_bytes(runs["number"][n][i], runs["none"][n][i])
+    assert not same_bytes(runs["list"]["ms"][5], runs["none"]["ms"][5])
+    for bad in (seeds[:-1], seeds + [1], []):
+        with pytest.raises(ValueError, match="seed"):
+            adam8(k, one, seed=bad)
+
+
+def test_every_field_of_every_layer_rounds_with_random_bits_of_its_own():
+    """The same bits for element i of all layers would add their rounding errors up instead of averaging them."""
+    import dataclasses
+    from dataflow_b200.models.families import resolve_family
+    from dataflow_b200.run.driver import Trainer, synthetic_rounds
+    cfg = dataclasses.replace(resolve_family("llama3").presets["tiny"](), dtype_policy="bf16_8bit")
+
+    def seeds_of_two_steps():
+        K, calls = resolve_kernels(kernel_set="eager"), []
+        step = K.lowbit.adamw_multi_step
+
+        def recorded(ws, *a, seed=None, **kw):
+            calls.extend(seed if isinstance(seed, list) else [seed] * len(ws))
+            return step(ws, *a, seed=seed, **kw)
+        K.lowbit.adamw_multi_step = recorded
+        tr = Trainer("llama3", cfg, budget_gib=None, device=None, hyper={"lr": 1e-3}, seed=0, kernels=K)
+        for s in range(2):
+            tr.step(synthetic_rounds(cfg, tr.rounds, tr.T, 64, 1, s))
+        tr.close()
+        return calls
+    calls = seeds_of_two_steps()
+    assert None not in calls and len(set(calls)) == len(calls) == 2 * (5 * cfg.n_layers + 1 + 2 + cfg.n_layers)
+    assert calls == seeds_of_two_steps()
