@@ -244,10 +244,14 @@ def adamw_multi_step(ws, gs, ms, vs, lr, beta1=0.9, beta2=0.95, eps=1e-8, wds=0.
     bits8 = bool(n) and ms[0].dtype == torch.float8_e4m3fn
     _need(not bits8 or (m_scales is not None and v_scales is not None), "adamw_multi_step: 8-bit moments come with m_scales and v_scales")
     _need(bits8 or (m_scales is None and v_scales is None) or not n, "adamw_multi_step: scales belong to 8-bit moments")
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), l is not gs)
-                   for l in (ws, gs, ms, vs, masters, los, m_scales, v_scales) if l is not None for t in l if t.numel())
-    for (_, end, a), (start, _, b) in zip(spans, spans[1:]):
-        _need(start >= end or not (a or b), "adamw_multi_step: a tensor that is written appears twice or overlaps another")
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), written)
+                   for l, written in ((ws, True), (gs, False), (ms, True), (vs, True), (masters, True), (los, True), (m_scales, True), (v_scales, True))
+                   if l is not None for t in l if t.numel())
+    end_written = end_any = 0               # how far the spans so far reach
+    for start, end, written in spans:
+        _need(start >= end_written and (not written or start >= end_any),
+              "adamw_multi_step: a tensor that is written appears twice or overlaps another")
+        end_written, end_any = max(end_written, end if written else 0), max(end_any, end)
     bc1, bc2 = 1 - beta1 ** int(step), 1 - beta2 ** int(step)
     seeds = list(seed) if isinstance(seed, (list, tuple)) else [int(step) if seed is None else int(seed)] * n
     _need(len(seeds) == n, "adamw_multi_step: seed has one entry per tensor")

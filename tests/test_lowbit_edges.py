@@ -200,3 +200,38 @@ def test_every_field_of_every_layer_rounds_with_random_bits_of_its_own():
     calls = seeds_of_two_steps()
     assert None not in calls and len(set(calls)) == len(calls) == 2 * (5 * cfg.n_layers + 1 + 2 + cfg.n_layers)
     assert calls == seeds_of_two_steps()
+
+
+# ------------------------------------------------------------------ AdamW: overlaps that are not neighbours
+def overlapping_lists():
+    f = lambda n=128: torch.zeros(n)
+    big = torch.zeros(1024)
+    yield "a weight inside a long gradient, a short one between", ([f(512), f(), big[300:428]], [big[:512], big[100:228], f()], 3)
+    yield "a moment inside a long gradient, a short one between", ([f(512), f(), f()], [big[:512], big[100:228], f()], big[300:428])
+    yield "weights and gradients are one list", (None, None, 1)
+
+
+@pytest.mark.parametrize("name,args", list(overlapping_lists()), ids=[n for n, _ in overlapping_lists()])
+@pytest.mark.parametrize("where", ["plain lane", "extension"])
+def test_adamw_refuses_a_written_tensor_inside_a_longer_one(name, args, where):
+    from dataflow_b200.ops import lowbit, native_available
+    if where == "extension" and not native_available():
+        pytest.skip("extension not built")
+    K = plain() if where == "plain lane" else lowbit
+    ws, gs, last = args
+    if ws is None:
+        ws = gs = [torch.zeros(128)]
+        ms, vs = [torch.zeros(128)], [torch.zeros(128)]
+    else:
+        ms, vs = [torch.zeros(t.numel()) for t in ws], [torch.zeros(t.numel()) for t in ws]
+        if torch.is_tensor(last):
+            vs[-1] = last
+    with pytest.raises(ValueError, match="twice or overlaps"):
+        K.adamw_multi_step(ws, gs, ms, vs, 1e-3)
+
+
+def test_adamw_gradients_may_share_memory():
+    """They are only read."""
+    big, f = torch.ones(512), lambda n: torch.zeros(n)
+    ws = plain().adamw_multi_step([f(512), f(128), f(128)], [big, big[100:228], big[100:228]], [f(512), f(128), f(128)], [f(512), f(128), f(128)], 1e-3)
+    assert all((w < 0).all() for w in ws)
