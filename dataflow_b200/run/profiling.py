@@ -59,6 +59,8 @@ def profile_key(trainer, cfg) -> str:
                                               for k, v in dataclasses.asdict(cfg).items() if k not in ("n_layers", "grad_accum_rounds", "name")},
             "kernels": trainer.K.describe(), "kernel_build": _ops_build_id(), "torch": torch.__version__,
             "device": torch.cuda.get_device_name(trainer.device) if trainer.device is not None else "cpu"}
+    if trainer.linear_precision != "bf16":          # a hyper-parameter for some families; costs of other GEMMs
+        desc["linear_precision"] = trainer.linear_precision
     return hashlib.sha256(json.dumps(desc, sort_keys=True).encode()).hexdigest()[:20]
 
 

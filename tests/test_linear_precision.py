@@ -113,3 +113,16 @@ def test_an_unknown_precision_is_refused_where_it_is_written():
             F.linear(x, w, p)
         with pytest.raises(ValueError, match="linear_precision"):
             F.swiglu_mlp(x, torch.zeros(64, 64), torch.zeros(32, 5), p)
+
+
+def test_measured_costs_of_one_precision_are_not_used_for_another():
+    """The cost cache's key: the precision is a hyper-parameter of the llama-like families, not a field of their configuration."""
+    from dataflow_b200.run.profiling import profile_key
+    keys = {}
+    for family in ("llama3", "dsv32"):
+        cfg = resolve_family(family).presets["tiny"]()
+        for p in (None, "bf16", "fp8", "mxfp4"):
+            tr = Trainer(family, cfg, budget_gib=None, device=None, hyper={"linear_precision": p} if p else None, recompute=False, init=False)
+            keys[family, p] = profile_key(tr, tr.cfg)
+            tr.close()
+        assert keys[family, None] == keys[family, "bf16"] and len({keys[family, p] for p in ("bf16", "fp8", "mxfp4")}) == 3
