@@ -7,8 +7,8 @@
 // of e4m3's 6 to 12 % spacing, so rounding to nearest would never let it fall again.  The random bits are a hash of (element
 // index, seed).  A positive r keeps at least the smallest code.  The update itself uses the unrounded moments.
 //
-// The kernel moves 10 bytes per element with 8-bit moments (28 with fp32 moments and a master) and is bound by memory: 8 bits 372 us
-// at 218M parameters, 0.9 of the copy rate with the arithmetic close behind (45 instructions an element, issue slots 73 % busy);
+// The kernel moves 10 bytes per element with 8-bit moments (28 with fp32 moments and a master) and is bound by memory: 8 bits 377 us
+// at 218M parameters, 0.89 of the copy rate with the arithmetic close behind (45 instructions an element, issue slots 73 % busy);
 // 32 bits 175 us at 42M, the copy rate.  A block takes consecutive elements of one tensor, a thread eight or (8-bit moments) sixteen
 // of them, so that eight lanes share a scale.  Tensors travel as a table in the kernel's parameters (no copy, no device-side table
 // that a captured graph would share); a block finds its tensor by bisection.
@@ -41,7 +41,8 @@ struct Args {
   AdamHyper h;
 };
 
-// 32-bit integer mixer: two rounds of xor-shift and multiply
+// 32-bit integer mixer: two rounds of xor-shift and multiply; shifts and factors from C. Wellons, "Prospecting for Hash Functions"
+// (2018), found there by a search for the least bias between input and output bits
 DFB_DEVICE uint32_t mix32(uint32_t x) {
   x ^= x >> 16;
   x *= 0x7feb352du;

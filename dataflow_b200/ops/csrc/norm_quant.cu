@@ -257,7 +257,8 @@ int launch(const NormArgs& a, int num_sms, cudaStream_t s) {
   const long long rows = MX ? (a.rows + 127) / 128 * 128 : a.rows;      // with the padding of the scale tiles
   if (rows > 0x7fffffffLL) return -3;
   const int nvec = a.cols >> 3;
-  // as many blocks as stay resident: 1024 threads per SM
+  // Blocks for 1024 threads per SM: all resident where a thread holds at most 16 columns; with more (108 to 149 registers) an SM holds
+  // 256 to 512 threads at a time and the other blocks follow, each walking its own rows.
   auto go = [&](auto kernel, int threads, int rows_per_block) {
     const long long need = (rows + rows_per_block - 1) / rows_per_block, fit = static_cast<long long>(num_sms) * (1024 / threads);
     kernel<<<static_cast<unsigned>(need < fit ? need : fit), threads, 0, s>>>(a);

@@ -185,7 +185,8 @@ def rmsnorm_mxfp4(x, w, eps: float = 1e-5, residual=None, rstd=None, h_out=None)
 
 # ------------------------------------------------------------------ AdamW over many tensors
 def _mix32(x):
-    """32-bit integer mixer (two xor-shift-multiply rounds), on int64 tensors that hold values below 2^32."""
+    """32-bit integer mixer (two xor-shift-multiply rounds; shifts and factors from C. Wellons, "Prospecting for Hash Functions", 2018),
+    on int64 tensors that hold values below 2^32."""
     x = x ^ (x >> 16)
     x = (x * 0x7FEB352D) & 0xFFFFFFFF
     x = x ^ (x >> 15)
