@@ -235,3 +235,149 @@ def test_adamw_gradients_may_share_memory():
     big, f = torch.ones(512), lambda n: torch.zeros(n)
     ws = plain().adamw_multi_step([f(512), f(128), f(128)], [big, big[100:228], big[100:228]], [f(512), f(128), f(128)], [f(512), f(128), f(128)], 1e-3)
     assert all((w < 0).all() for w in ws)
+
+
+# ------------------------------------------------------------------ blocks that walk on
+def poison():
+    """Freed memory that is neither zero nor what an earlier call left."""
+    junk = [torch.full((n << 20,), 0xA5, dtype=U8, device="cuda") for n in (256, 64, 64, 8, 2, 1, 1, 1)]
+    torch.cuda.synchronize()
+    del junk
+
+
+def sm_count():
+    return torch.cuda.get_device_properties(0).multi_processor_count
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("off", [0, 8], ids=["on32", "on16"])
+@pytest.mark.parametrize("cols", [96, 256, 512, 1024, 2048, 4096, 8192, 16384])
+@pytest.mark.parametrize("fmt", ["fp8", "mxfp4"])
+def test_norm_rows_behind_the_first_of_a_block(fmt, cols, off):
+    """A block holds the next row's loads while it works on one and comes back for more rows when the matrix has more than the grid:
+    every row, its codes, scales (raw tiles, padding included), stream and statistic are those of slices that no block walks over."""
+    k = lane("cuda")
+    fn = k.rmsnorm_fp8 if fmt == "fp8" else k.rmsnorm_mxfp4
+    # threads of a row: one warp up to 1024 columns, else 128, 256 or 512 (twice as many in the 16-byte form); 1024 an SM at once
+    threads = 32 if cols <= 1024 else {2048: 128, 4096: 128, 8192: 256, 16384: 512}[cols]
+    rows = 2 * sm_count() * (1024 // threads) + sm_count() * (512 // threads) + 77
+    g = torch.Generator(device="cuda").manual_seed(cols + off)
+    big = torch.randn(rows, cols + 16, device="cuda", generator=g).to(BF)
+    res = torch.randn(rows, cols + 16, device="cuda", generator=g).to(BF)
+    w = (1 + 0.1 * torch.randn(cols, device="cuda", generator=g)).to(BF)
+    x, r = big[:, off:off + cols], res[:, off:off + cols]
+    for residual in (None, r):
+        poison()
+        got = fn(x, w, residual=residual)
+        given = fn(x, w, residual=residual, rstd=got[3])
+        for a in range(0, rows, 256):
+            b = min(a + 256, rows)
+            want = fn(x[a:b], w, residual=None if residual is None else residual[a:b])
+            for full, part in ((got, want), (given, want)):
+                assert same_bytes(full[0][a:b], part[0]) and same_bytes(full[2][a:b], part[2]) and torch.equal(full[3][a:b], part[3])
+                if fmt == "fp8":
+                    assert torch.equal(full[1][a:b], part[1])
+                else:
+                    assert torch.equal(full[1][a // 128:a // 128 + part[1].shape[0]], part[1])
+    # the sum in place of the residual, rows already on their way included
+    out = res.clone()
+    q, s, h, rstd = fn(x, w, residual=out[:, off:off + cols], h_out=out[:, off:off + cols])
+    assert same_bytes(q, got[0]) and torch.equal(s, got[1]) and same_bytes(h, got[2]) and torch.equal(rstd, got[3])
+    assert torch.equal(out[:, :off], res[:, :off]) and torch.equal(out[:, off + cols:], res[:, off + cols:])
+
+
+def adam_lists(form, gdt, sizes, seed, starts):
+    """Lists with 8-bit moments; ``starts``: bytes by which weights, gradients and masters, and states, miss a multiple of 512."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    wide, state = starts
+
+    def at(t, miss):
+        off = miss // t.element_size()
+        buf = torch.empty(off + t.numel(), dtype=t.dtype, device="cuda")
+        buf[off:] = t
+        assert (buf[off:].data_ptr() - miss) % 512 == 0
+        return buf[off:]
+    rnd = lambda n, s: torch.randn(n, device="cuda", generator=g) * s
+    st = {n: [] for n in ("ws", "gs", "ms", "vs", "m_scales", "v_scales")}
+    for n in sizes:
+        full = rnd(n, 0.05)
+        if form == "fp32":
+            st["ws"].append(at(full, wide))
+        elif form == "split":
+            hi, lo = E.split_master_cut(full)
+            st["ws"].append(at(hi, wide))
+            st.setdefault("los", []).append(at(lo, wide))
+        else:
+            st["ws"].append(at(full.to(BF), wide))
+            if form == "master":
+                st.setdefault("masters", []).append(at(full, wide))
+        st["gs"].append(at(rnd(n, 1e-2).to(gdt), wide))
+        st["ms"].append(at(rnd(n, 60).to(F8), state))
+        st["vs"].append(at(rnd(n, 60).abs().to(F8), state))
+        for name in ("m_scales", "v_scales"):
+            st[name].append(1e-5 * (1 + torch.rand(-(-n // 128), device="cuda", generator=g)))
+    return st
+
+
+def adam_step(k, st, only=None):
+    pick = (lambda l: l) if only is None else (lambda l: [l[only]])
+    k.adamw_multi_step(*[pick(st[n]) for n in ("ws", "gs", "ms", "vs")], 1e-3, wds=0.1, step=3,
+                       **{n: pick(st[n]) for n in ("masters", "los", "m_scales", "v_scales") if n in st})
+
+
+# more elements than blocks of one group take: ragged ends, an end inside a block's 8192, one inside a group of 512, whole blocks
+def long_sizes():
+    least = 2 * sm_count() * 16 * 8192
+    return [least // 2 + 3, least // 2 + 8192 * 5 + 517, 8192 * 64, 300, 8192 * 3 + 128, 129, 1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gdt", [BF, F32], ids=["gbf16", "gfp32"])
+@pytest.mark.parametrize("form", ["bf16", "fp32", "master", "split"])
+@pytest.mark.parametrize("starts", [(0, 0), (16, 16), (0, 16), (16, 0), (2, 1), (32, 48)], ids=["aligned", "on16", "states16", "weights16", "odd", "by32"])
+def test_adamw_long_lists(form, gdt, starts):
+    """Lists of more than 2 x SMs x 16 x 8192 elements, where a block takes 8192 at a time with the next group on its way: every
+    element of every tensor as in a call on that tensor alone, which takes one group a block, from 512-byte starts."""
+    if starts[0] % 4 and (form in ("fp32", "master") or gdt == F32):
+        starts = (4, starts[1])
+    k, sizes = lane("cuda"), long_sizes()
+    st, one = adam_lists(form, gdt, sizes, 5, starts), adam_lists(form, gdt, sizes, 5, (0, 0))
+    assert sum(sizes) >= 2 * sm_count() * 16 * 8192 > max(sizes)
+    adam_step(k, st)
+    for i in range(len(sizes)):
+        adam_step(k, one, only=i)
+        for n in st:
+            assert same_bytes(st[n][i], one[n][i]), (n, i)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("starts", [(0, 0), (16, 16)], ids=["on32", "on16"])
+def test_adamw_long_lists_against_the_plain_lane(starts):
+    """The state to the bit, and the weights by the definition in 64 bits on the plain lane's unrounded arithmetic: lr times a
+    quotient that is off by at most 8 roundings and the approximate reciprocal (2^-23), and 4 roundings of the weight."""
+    sizes = long_sizes()
+    st, ref = adam_lists("master", BF, sizes, 6, starts), adam_lists("master", BF, sizes, 6, (0, 0))
+    old = [t.clone() for t in ref["masters"]]
+    adam_step(lane("cuda"), st)
+    adam_step(plain(), ref)
+    for i in range(len(sizes)):
+        for n in ("ms", "vs", "m_scales", "v_scales"):
+            assert same_bytes(st[n][i], ref[n][i]), (n, i)
+        moved = (ref["masters"][i].double() - old[i].double()).abs()
+        err = (st["masters"][i].double() - ref["masters"][i].double()).abs()
+        assert (err <= 16 * 2.0 ** -24 * moved + 8 * 2.0 ** -24 * old[i].double().abs()).all()
+        assert torch.equal(st["ws"][i], st["masters"][i].to(BF))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["bf16", "fp32", "master", "split"])
+@pytest.mark.parametrize("starts", [(16, 16), (0, 16), (16, 0), (48, 32)], ids=["on16", "states16", "weights16", "by16"])
+def test_adamw_short_lists_that_start_on_16_bytes(form, starts):
+    """Weights on 16 but not 32 bytes with states on 16: the kernel's 16-byte form, which a common offset of elements never meets."""
+    k, sizes = lane("cuda"), [512 * 7, 4096, 512 + 77, 128]
+    st, one = adam_lists(form, BF, sizes, 7, starts), adam_lists(form, BF, sizes, 7, (0, 0))
+    adam_step(k, st)
+    adam_step(k, one)
+    for n in st:
+        for a, b in zip(st[n], one[n]):
+            assert same_bytes(a, b), n
