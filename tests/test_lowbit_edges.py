@@ -381,3 +381,27 @@ def test_adamw_short_lists_that_start_on_16_bytes(form, starts):
     for n in st:
         for a, b in zip(st[n], one[n]):
             assert same_bytes(a, b), n
+
+
+# ------------------------------------------------------------------ the norm's 8-bit operand in the 8-bit product
+@pytest.mark.parametrize("dev", LANES)
+@pytest.mark.parametrize("M,K,N", [(1, 32, 16), (130, 208, 72), (300, 1040, 264)])
+def test_norm_to_fp8_feeds_the_fp8_product(dev, M, K, N):
+    """Codes and scales go into ``linear_fp8`` as they are: against 64 bits on the same codes, K products of 8-bit codes summed in 32
+    bits (each addition off by at most 2^-23 of the running magnitude), two scalings, one rounding to bf16."""
+    ks = resolve_kernels(kernel_set="eager" if dev == "cpu" else None)
+    g = torch.Generator().manual_seed(M + N)
+    x, res = torch.randn(M, K, generator=g).to(BF).to(dev), torch.randn(M, K, generator=g).to(BF).to(dev)
+    gain, w = (1 + 0.1 * torch.randn(K, generator=g)).to(BF).to(dev), (torch.randn(N, K, generator=g) * K ** -0.5).to(BF).to(dev)
+    q, s, h, rstd = ks.lowbit.rmsnorm_fp8(x, gain, residual=res)
+    wq, sw = ks.quant_fp8_rowwise(w)
+    y = ks.linear_fp8(q, s, wq, sw)
+    A, B = q.double() * s.double()[:, None], wq.double() * sw.double()[:, None]
+    want = A @ B.t()
+    bound = ((K + 2) * 2.0 ** -23 + 3 * 2.0 ** -24) * (A.abs() @ B.abs().t()) + torch.finfo(BF).eps / 2 * want.abs()
+    assert y.dtype == BF and ((y.double() - want).abs() <= bound).all()
+    # and what the codes stand for is the norm of the sum, off by half a code (2^-4 of the value, or of the smallest normal code)
+    h64 = (x.float() + res.float()).to(BF).double()
+    y64 = h64 / torch.sqrt(h64.square().mean(-1, keepdim=True) + 1e-5) * gain.double()
+    assert torch.equal(h.double(), h64)
+    assert ((A - y64).abs() <= (2.0 ** -4 + (K + 16) * 2.0 ** -24) * y64.abs() + s.double()[:, None] * 2.0 ** -10).all()
