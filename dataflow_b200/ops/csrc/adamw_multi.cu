@@ -7,11 +7,11 @@
 // of e4m3's 6 to 12 % spacing, so rounding to nearest would never let it fall again.  The random bits are a hash of (element
 // index, seed).  A positive r keeps at least the smallest code.  The update itself uses the unrounded moments.
 //
-// The kernel moves 10 bytes per element with 8-bit moments (28 with fp32 moments and a master) and is bound by memory: 8 bits 377 us
-// at 218M parameters, 0.89 of the copy rate with the arithmetic close behind (45 instructions an element, issue slots 73 % busy);
-// 32 bits 175 us at 42M, the copy rate.  A block takes consecutive elements of one tensor, a thread eight or (8-bit moments) sixteen
-// of them, so that eight lanes share a scale.  Tensors travel as a table in the kernel's parameters (no copy, no device-side table
-// that a captured graph would share); a block finds its tensor by bisection.
+// The kernel moves 10 bytes per element with 8-bit moments (28 with fp32 moments and a master) and is bound by memory: 8 bits 378 us
+// at 218M parameters, 0.89 of the copy rate with the arithmetic close behind (47 instructions an element, issue slots 73 % busy; 6 us of
+// it for roots that are right at every size); 32 bits 175 us at 42M, the copy rate.  A block takes consecutive elements of one tensor, a
+// thread eight or (8-bit moments) sixteen of them, so that eight lanes share a scale.  Tensors travel as a table in the kernel's
+// parameters (no copy, no device-side table that a captured graph would share); a block finds its tensor by bisection.
 #include "lowbit.h"
 #include "lowbit_common.cuh"
 
